@@ -406,6 +406,146 @@ int zdraw_hip_run_chain_attn_enc(void* batch, const ZdrawHipChainAttnBuffers* bu
                                  const ZdrawHipChainAttnWeights* weights,
                                  const ZdrawHipChainAttnParams* params);
 
+/* ---- attention under masks ---------------------------------------------------
+ * No counterpart in the reference, whose causal and grouped-query attention (the text
+ * encoder's, runtime/attention.zig:40-113) runs on the CPU. Row i of a document of nq query
+ * rows and nk keys sees
+ *     every key                                     causal == 0
+ *     keys j < max(prefix, i + 1 + nk - nq)         causal != 0 (the last query stands on the last key)
+ * and its output is softmax(s) v over those keys, with
+ *     s = scale q.k;  s = softcap tanh(s / softcap);  s = s - slopes[head] |i + nk - nq - j|
+ * (the cap where softcap > 0, the bias where slopes are given). A row that sees no key gets
+ * zeros. Query head h reads key head h / (heads / kv_heads).
+ * A segment is one document of q_tokens and k_tokens, or `documents` packed ones between
+ * borders in GPU memory; rows and keys outside of every document (behind the last border)
+ * take no part, and the output rows there stay as they were. (Padded segments of different
+ * length: one document each.) Borders are held to the segment; they have to ascend, or rows
+ * get other documents' keys.
+ * K and V rows that a query row does not see may hold anything, infinities and NaN too.
+ * Q, K, V and the output have one 16-bit type; scores, sums and the running maximum are f32,
+ * probabilities are rounded to the type of V. Strides in elements: [0] between segments, [1] between tokens, [2]
+ * between heads; multiples of 8, those of the inputs may be 0. Outside of what is described the
+ * calls return 1 (head_dim other than 128, f32 operands, 2^24 rows or more) or 2. No queries (q_tokens or
+ * batch 0) is no error and enqueues nothing; without keys (k_tokens 0) k and v may be NULL. */
+typedef struct ZdrawHipMaskedAttn {
+    uint64_t q_off, k_off, v_off, out_off; /* byte offsets into the buffers, multiples of 16 */
+    uint64_t q_stride[3];
+    uint64_t k_stride[3];
+    uint64_t v_stride[3];
+    uint64_t out_stride[3];
+    uint32_t batch;     /* segments */
+    uint32_t q_tokens;  /* query rows of a segment */
+    uint32_t k_tokens;  /* keys of a segment */
+    uint32_t heads, kv_heads, head_dim;
+    uint32_t dtype;     /* ZDRAW_HIP_F16 or ZDRAW_HIP_BF16 */
+    uint32_t causal;
+    uint32_t documents; /* packed documents of a segment; 0 = the segment is one */
+    float scale;        /* 0 = 1 / sqrt(head_dim) */
+    float softcap;      /* 0 = none */
+    uint32_t reserved;  /* 0 */
+} ZdrawHipMaskedAttn;
+
+typedef struct ZdrawHipMaskOperands {
+    void* q_starts;  /* u32 [batch][documents + 1]: first query row of each document, and the end; NULL without documents */
+    void* k_starts;  /* the same for the keys; NULL = q_starts (then q_tokens == k_tokens) */
+    void* prefix;    /* u32 [batch][max(documents, 1)]: keys that all of a document's rows see (causal only), or NULL */
+    void* slopes;    /* f32 [heads], or NULL */
+    void* workspace; /* room for joined parts (zdraw_hip_attention_masked_workspace), or NULL: the queue's own */
+} ZdrawHipMaskOperands;
+
+/* A call with few rows splits the keys over the GPU and joins the parts, through the queue's scratch slots 3 and 4 or
+ * through ops->workspace. A call under capture takes the queue's slots never (a larger call may replace them while the
+ * graph lives): without a workspace it runs unsplit, slower where rows are few. Two graphs that may run at the same time
+ * need a workspace each. */
+int zdraw_hip_run_attention_masked_enc(void* batch, void* q, void* k, void* v, void* out, const ZdrawHipMaskedAttn* params,
+                                       const ZdrawHipMaskOperands* ops);
+/* Same, on a queue, blocking until complete. ops may be NULL in both. */
+int zdraw_hip_run_attention_masked(void* queue, void* q, void* k, void* v, void* out, const ZdrawHipMaskedAttn* params,
+                                   const ZdrawHipMaskOperands* ops);
+/* Bytes of workspace that the call takes on this queue's device (0: none). Host arithmetic only. */
+size_t zdraw_hip_attention_masked_workspace(void* queue, const ZdrawHipMaskedAttn* params);
+
+/* ---- attention of a batch over a shared prefix ---------------------------------
+ * No counterpart in the reference. The rows of `requests` requests see all prefix_tokens keys of
+ * one prefix (a long prompt, the kept keys and values of a reference image), which are read
+ * once for all of them where rows are few, and the first lens[r] keys of their own cache:
+ *     every one of them                         causal == 0
+ *     own keys j <= t + lens[r] - q_lens[r]     causal != 0, for row t of q_lens[r]
+ * Scores, cap, bias and types as above; the distance of the bias counts the prefix ahead of the
+ * own keys. The own cache is [requests][capacity] rows, or pages of page_tokens rows (a power of
+ * two from 4 on) in any order: k_stride[0] and v_stride[0] are then between pages, and
+ * page_table[r][j / page_tokens] names the page of own key j. Only the pages of the first
+ * lens[r] keys are looked up; a number past the pool is held to its last page. lens and q_lens
+ * are held to capacity and q_tokens. Output rows t >= q_lens[r] stay as they were. No requests
+ * or queries is no error; without a prefix (prefix_tokens 0) or own keys (capacity 0) their buffers may be NULL. */
+typedef struct ZdrawHipSharedAttn {
+    uint64_t q_off, out_off, prefix_k_off, prefix_v_off, k_off, v_off;
+    uint64_t q_stride[3], out_stride[3];             /* between requests, tokens, heads */
+    uint64_t prefix_k_stride[2], prefix_v_stride[2]; /* between tokens, heads */
+    uint64_t k_stride[3], v_stride[3];               /* between requests (pages), tokens, heads */
+    uint32_t requests, q_tokens, prefix_tokens;
+    uint32_t capacity;    /* own keys that a request has room for */
+    uint32_t page_tokens; /* 0 = no pages */
+    uint32_t pages;       /* pages of the pool */
+    uint32_t heads, kv_heads, head_dim, dtype, causal;
+    float scale, softcap;
+    uint32_t reserved;    /* 0 */
+} ZdrawHipSharedAttn;
+
+typedef struct ZdrawHipSharedOperands {
+    void* lens;       /* u32 [requests]; NULL only with capacity 0 */
+    void* q_lens;     /* u32 [requests], or NULL: q_tokens rows each */
+    void* page_table; /* u32 [requests][ceil(capacity / page_tokens)]; NULL without pages */
+    void* slopes;     /* f32 [heads], or NULL */
+    void* workspace;  /* as in ZdrawHipMaskOperands */
+} ZdrawHipSharedOperands;
+
+int zdraw_hip_run_attention_shared_enc(void* batch, void* q, void* prefix_k, void* prefix_v, void* k, void* v, void* out,
+                                       const ZdrawHipSharedAttn* params, const ZdrawHipSharedOperands* ops);
+int zdraw_hip_run_attention_shared(void* queue, void* q, void* prefix_k, void* prefix_v, void* k, void* v, void* out,
+                                   const ZdrawHipSharedAttn* params, const ZdrawHipSharedOperands* ops);
+size_t zdraw_hip_attention_shared_workspace(void* queue, const ZdrawHipSharedAttn* params);
+
+/* ---- cache append ---------------------------------------------------------------
+ * Key and value rows t < counts[r] of every request go to places starts[r] + t of its cache (laid out as above): K
+ * rows RMS-normalised where k_weight is given (y = x rsqrt(mean x^2 + eps) w), rotated and rounded to the cache's type,
+ * V rows rounded. Query rows, where heads > 0, take the same way (q_weight) to q_out. The rotation reads row
+ * position_base + starts[r] + t of the cos and sin tables, f32 [rope_rows][128] (a position past them reads the last
+ * row): z = y cos + turn(y) sin, where turn takes (y0, y1) to (-y1, y0) on adjacent pairs (ZDRAW_HIP_ROTATE_PAIRS: the
+ * krms_rope form, klein/zflux2_glue_shader.zig:61-83) or on the pairs (y_i, y_{i + 64}) (ZDRAW_HIP_ROTATE_HALVES: the
+ * text encoder's). Rows past `capacity`, or on a page number past the pool, are not kept; no other place is written.
+ * Rows that the table sends to one place leave any one of them there. The counts of what a cache holds stay with the
+ * caller: starts is not changed. */
+enum { ZDRAW_HIP_ROTATE_NONE = 0, ZDRAW_HIP_ROTATE_PAIRS = 1, ZDRAW_HIP_ROTATE_HALVES = 2 };
+typedef struct ZdrawHipKvAppend {
+    uint64_t q_off, k_off, v_off, q_out_off, cache_k_off, cache_v_off;
+    uint64_t q_stride[3], k_stride[3], v_stride[3], q_out_stride[3]; /* between requests, tokens, heads */
+    uint64_t cache_k_stride[3], cache_v_stride[3];                   /* between requests (pages), tokens, heads */
+    uint32_t requests, tokens;                     /* new rows of a request, at most */
+    uint32_t capacity, page_tokens, pages;         /* as in ZdrawHipSharedAttn */
+    uint32_t heads;                                /* query heads; 0 = no query rows (q and q_out NULL) */
+    uint32_t kv_heads, head_dim;
+    uint32_t in_dtype;                             /* of q, k, v: ZDRAW_HIP_F32, F16 or BF16 */
+    uint32_t dtype;                                /* of q_out and the cache: ZDRAW_HIP_F16 or BF16 */
+    uint32_t rotation, rope_rows, position_base;
+    float eps;
+} ZdrawHipKvAppend;
+
+typedef struct ZdrawHipAppendOperands {
+    void* starts;     /* u32 [requests] */
+    void* counts;     /* u32 [requests], or NULL: `tokens` rows each */
+    void* page_table; /* u32 [requests][ceil(capacity / page_tokens)]; NULL without pages */
+    void* q_weight;   /* f32 [128], or NULL: no norm */
+    void* k_weight;
+    void* rope_cos;   /* f32 [rope_rows][128]; NULL without rotation */
+    void* rope_sin;
+} ZdrawHipAppendOperands;
+
+int zdraw_hip_run_kv_append_enc(void* batch, void* q, void* k, void* v, void* q_out, void* cache_k, void* cache_v,
+                                const ZdrawHipKvAppend* params, const ZdrawHipAppendOperands* ops);
+int zdraw_hip_run_kv_append(void* queue, void* q, void* k, void* v, void* q_out, void* cache_k, void* cache_v,
+                            const ZdrawHipKvAppend* params, const ZdrawHipAppendOperands* ops);
+
 /* ---- scratch slots (metal_c.zig:321-325) ----------------------------------
  * The reference's process-lifetime, grow-only slots, for callers that keep their own
  * intermediates in them: (re)allocated only to grow, filled at (re)allocation with 0x00
@@ -471,7 +611,9 @@ int zdraw_hip_zimage_axis_lens(uint64_t table_bytes, const uint64_t* base, const
  * shared structs as this library was compiled. which: 0 = ZdrawAttnParams,
  * 1 = ZdrawHipAttnExt, 2 = ZdrawHipQkOperands, 3 = ZdrawGemmParams,
  * 4 = ZdrawHipGemmExt, 5 = ZdrawQkNormParams, 6 = ZdrawHipChainAttnBuffers,
- * 7 = ZdrawHipChainAttnWeights, 8 = ZdrawHipChainAttnParams. */
+ * 7 = ZdrawHipChainAttnWeights, 8 = ZdrawHipChainAttnParams, 9 = ZdrawHipMaskedAttn,
+ * 10 = ZdrawHipMaskOperands, 11 = ZdrawHipSharedAttn, 12 = ZdrawHipSharedOperands,
+ * 13 = ZdrawHipKvAppend, 14 = ZdrawHipAppendOperands. */
 size_t zdraw_hip_abi_sizeof(int which);
 /* Last error text of this thread's most recent failing call ("" if none). */
 const char* zdraw_hip_last_error(void);
@@ -485,6 +627,12 @@ const char* zdraw_hip_last_error(void);
 #define ZDRAW_HIP_ABI_CHAIN_ATTN_BUFFERS_SIZE 48
 #define ZDRAW_HIP_ABI_CHAIN_ATTN_WEIGHTS_SIZE 64
 #define ZDRAW_HIP_ABI_CHAIN_ATTN_PARAMS_SIZE 240
+#define ZDRAW_HIP_ABI_MASKED_ATTN_SIZE 176
+#define ZDRAW_HIP_ABI_MASK_OPERANDS_SIZE 40
+#define ZDRAW_HIP_ABI_SHARED_ATTN_SIZE 232
+#define ZDRAW_HIP_ABI_SHARED_OPERANDS_SIZE 40
+#define ZDRAW_HIP_ABI_KV_APPEND_SIZE 248
+#define ZDRAW_HIP_ABI_APPEND_OPERANDS_SIZE 56
 
 #ifdef __cplusplus
 }

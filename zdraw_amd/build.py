@@ -43,7 +43,7 @@ def build_hip(verbose: bool = False, out: str | None = None, extra_flags=()) -> 
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     target = out or HIP_LIB
     tag = "" if out is None else "." + os.path.basename(out)
-    srcs = [os.path.join(CSRC, f) for f in ("attn_fwd.hip", "attn_wide.hip", "qk_prepass.hip", "gemm_half.hip", "bridge.hip")]
+    srcs = [os.path.join(CSRC, f) for f in ("attn_fwd.hip", "attn_wide.hip", "attn_masked.hip", "kv_append.hip", "qk_prepass.hip", "gemm_half.hip", "bridge.hip")]
     from concurrent.futures import ThreadPoolExecutor
     objs = [os.path.join(LIBDIR, os.path.basename(src) + tag + ".o") for src in srcs]
     with ThreadPoolExecutor(max_workers=min(len(srcs), os.cpu_count() or 1)) as pool:  # one hipcc per source file
@@ -335,7 +335,7 @@ def build_host(verbose: bool = False) -> str:
 def check_hand_scheduled_kernels(verbose: bool = False):
     """The GEMM's hand-placed MFMAs and its M0 held across loads are safe only as long as the
     compiler puts nothing of its own in between: a toolchain that does fails the build here."""
-    files = [os.path.join(CSRC, f) for f in ("attn_fwd.hip", "attn_wide.hip", "gemm_half.hip", "qk_prepass.hip")]
+    files = [os.path.join(CSRC, f) for f in ("attn_fwd.hip", "attn_wide.hip", "gemm_half.hip", "qk_prepass.hip", "attn_masked.hip", "kv_append.hip")]
     from concurrent.futures import ThreadPoolExecutor
     with ThreadPoolExecutor(max_workers=len(files)) as pool:  # one compilation per file, kept for all checks
         list(pool.map(_device_asm, files))

@@ -11,6 +11,7 @@
 #include "../../include/zdraw_hip_measure.h"
 #include "attn_kernel.h"
 #include "gemm_kernel.h"
+#include "masked_kernel.h"
 
 #include <hip/hip_runtime.h>
 
@@ -44,6 +45,12 @@ static_assert(sizeof(ZdrawQkNormParams) == ZDRAW_HIP_ABI_QK_NORM_PARAMS_SIZE, "Q
 static_assert(sizeof(ZdrawHipChainAttnBuffers) == ZDRAW_HIP_ABI_CHAIN_ATTN_BUFFERS_SIZE, "ChainAttnBuffers ABI drift");
 static_assert(sizeof(ZdrawHipChainAttnWeights) == ZDRAW_HIP_ABI_CHAIN_ATTN_WEIGHTS_SIZE, "ChainAttnWeights ABI drift");
 static_assert(sizeof(ZdrawHipChainAttnParams) == ZDRAW_HIP_ABI_CHAIN_ATTN_PARAMS_SIZE, "ChainAttnParams ABI drift");
+static_assert(sizeof(ZdrawHipMaskedAttn) == ZDRAW_HIP_ABI_MASKED_ATTN_SIZE, "MaskedAttn ABI drift");
+static_assert(sizeof(ZdrawHipMaskOperands) == ZDRAW_HIP_ABI_MASK_OPERANDS_SIZE, "MaskOperands ABI drift");
+static_assert(sizeof(ZdrawHipSharedAttn) == ZDRAW_HIP_ABI_SHARED_ATTN_SIZE, "SharedAttn ABI drift");
+static_assert(sizeof(ZdrawHipSharedOperands) == ZDRAW_HIP_ABI_SHARED_OPERANDS_SIZE, "SharedOperands ABI drift");
+static_assert(sizeof(ZdrawHipKvAppend) == ZDRAW_HIP_ABI_KV_APPEND_SIZE, "KvAppend ABI drift");
+static_assert(sizeof(ZdrawHipAppendOperands) == ZDRAW_HIP_ABI_APPEND_OPERANDS_SIZE, "AppendOperands ABI drift");
 
 namespace {
 
@@ -1160,6 +1167,7 @@ void* zdraw_hip_create_device(void) {
     // their code), and this device's address of the no-allocation entry's scratch array.
     if (!g_setup_done) {
         hipError_t e = attention_setup();
+        if (e == hipSuccess) e = masked_setup();
         if (e != hipSuccess) {
             set_err("attention_setup: %s", hipGetErrorString(e));
             return nullptr;
@@ -1887,6 +1895,547 @@ int zdraw_hip_run_chain_attn_enc(void* batch, const ZdrawHipChainAttnBuffers* bu
     return enqueue_gemm(bufs->mix, w->proj, bufs->attn, &p->proj, &gx, b->queue, plan.args.o16 != nullptr);
 }
 
+} // extern "C"
+
+// ------------------------------------------------ attention under masks, over a shared prefix; cache append
+namespace {
+
+// A strided operand [n0][n1][n2][128] checked against its buffer: every row starts at a multiple of 16 bytes and lies
+// inside. `written`: rows may not lie on top of each other.
+const char* check_rows(void* handle, uint64_t off, const uint64_t* stride, const uint64_t n[3], size_t es, bool written, const char* name) {
+    static thread_local char why[128];
+    const char* what = nullptr;
+    const Buffer* b = static_cast<Buffer*>(handle);
+    unsigned __int128 last = kHeadDim;
+    if (!b || !b->ptr) what = "null buffer";
+    else if ((uintptr_t)b->ptr % 16 != 0 || off % 16 != 0) what = "rows must start at multiples of 16 bytes";
+    for (int i = 0; i < 3 && !what; i++) {
+        if (n[i] <= 1) continue;
+        if (stride[i] % (16 / es) != 0) what = "strides must keep rows 16-byte aligned";
+        else if (stride[i] >= (1ull << 58)) what = "stride too large";
+        else if (written && stride[i] < (uint64_t)kHeadDim) what = "rows lie on top of each other";
+        last += (unsigned __int128)(n[i] - 1) * stride[i];
+    }
+    if (!what && (off > b->len || last * es > b->len - off)) what = "buffer too small for the declared shape";
+    if (!what) return nullptr;
+    snprintf(why, sizeof(why), "%s: %s", name, what);
+    return why;
+}
+
+// Strides in bytes; those of an axis with one entry are never used.
+void byte_strides(int64_t out[3], const uint64_t* stride, const uint64_t n[3], size_t es) {
+    for (int i = 0; i < 3; i++) out[i] = n[i] > 1 ? (int64_t)(stride[i] * es) : 0;
+}
+
+bool need_u32(const void* handle, uint64_t count) {
+    const Buffer* b = static_cast<const Buffer*>(handle);
+    return b && b->ptr && (uintptr_t)b->ptr % 4 == 0 && b->len / 4 >= count;
+}
+
+const unsigned* u32_of(void* handle) { return handle ? static_cast<const unsigned*>(static_cast<Buffer*>(handle)->ptr) : nullptr; }
+const float* f32_of(void* handle) { return handle ? static_cast<const float*>(static_cast<Buffer*>(handle)->ptr) : nullptr; }
+
+constexpr uint32_t kMaskMaxTokens = 1u << 24; // positions and row numbers are exact in f32
+
+// How the rows of a call are laid on workgroups (2 per CU). `split_ok`: there is room for parts.
+struct MaskLayout {
+    int by_keys, row_tiles, splits;
+};
+MaskLayout mask_layout(int64_t rows, int64_t groups, int64_t keys, int cus, bool split_ok) {
+    MaskLayout y;
+    const int64_t slots = 2 * (int64_t)cus;
+    const int64_t tiles32 = (rows + kMaskRowsByKeys - 1) / kMaskRowsByKeys * groups;
+    y.by_keys = rows <= kMaskRowsByKeys || tiles32 <= slots;
+    const int tr = y.by_keys ? kMaskRowsByKeys : kMaskRowsByWave;
+    y.row_tiles = (int)((rows + tr - 1) / tr);
+    const int64_t wgs = y.row_tiles * groups;
+    int64_t s = split_ok ? slots / wgs : 1;
+    s = std::min(s, (keys + 255) / 256);
+    y.splits = (int)std::max<int64_t>(1, std::min<int64_t>(s, 64));
+    return y;
+}
+
+int64_t job_rows(const MaskJob& j) { return (int64_t)j.workgroups * (j.by_keys ? kMaskRowsByKeys : kMaskRowsByWave); }
+
+int set_job(MaskJob* j, const MaskLayout& y, int seqs, int kv_heads, int64_t rows, int pooled) {
+    j->by_keys = y.by_keys;
+    j->seqs = seqs;
+    j->pooled = pooled;
+    j->rows = (int32_t)rows;
+    j->row_tiles = y.row_tiles;
+    j->splits = y.splits;
+    const int64_t wgs = (int64_t)seqs * kv_heads * y.row_tiles * y.splits;
+    if (wgs > 0x3fffffffLL) return unavailable("grid too large");
+    j->workgroups = (int32_t)wgs;
+    return ZDRAW_HIP_OK;
+}
+
+// The jobs of a call from its shape alone, and the bytes of room their parts take.
+int plan_masked_jobs(const ZdrawHipMaskedAttn* p, int cus, bool split_ok, MaskArgs* a, size_t* part_rows) {
+    const int64_t rows = (int64_t)p->q_tokens * (p->heads / p->kv_heads);
+    a->jobs = 1;
+    MaskJob& j = a->job[0];
+    j.spans = 1;
+    j.kind[0] = kRangeDocs;
+    const MaskLayout y = mask_layout(rows, (int64_t)p->batch * p->kv_heads, p->k_tokens, cus, split_ok);
+    const int rc = set_job(&j, y, (int)p->batch, (int)p->kv_heads, rows, 0);
+    if (rc != ZDRAW_HIP_OK) return rc;
+    a->direct = j.splits == 1;
+    *part_rows = a->direct ? 0 : (size_t)job_rows(j);
+    return ZDRAW_HIP_OK;
+}
+
+// A request's rows walk the prefix and then their own keys in one workgroup where they fill one and there are
+// workgroups enough; otherwise the prefix is walked once for the rows of all requests.
+int plan_shared_jobs(const ZdrawHipSharedAttn* p, int cus, bool split_ok, MaskArgs* a, size_t* part_rows) {
+    const int64_t rows = (int64_t)p->q_tokens * (p->heads / p->kv_heads);
+    const int64_t groups = (int64_t)p->requests * p->kv_heads;
+    MaskJob& j0 = a->job[0];
+    MaskJob& j1 = a->job[1];
+    int rc;
+    const bool both = p->prefix_tokens != 0 && p->capacity != 0;
+    const bool full = rows >= 64 && (rows + 127) / 128 * groups >= cus / 2;
+    if (!both || !split_ok || full) {
+        a->jobs = 1;
+        j0.spans = both ? 2 : 1;
+        j0.kind[0] = both || p->prefix_tokens != 0 ? kRangePrefix : kRangeOwn;
+        j0.kind[1] = kRangeOwn;
+        MaskLayout y = mask_layout(rows, groups, (int64_t)p->prefix_tokens + p->capacity, cus, split_ok && !both);
+        if ((rc = set_job(&j0, y, (int)p->requests, (int)p->kv_heads, rows, 0)) != ZDRAW_HIP_OK) return rc;
+        a->direct = j0.splits == 1;
+        *part_rows = a->direct ? 0 : (size_t)job_rows(j0);
+        return ZDRAW_HIP_OK;
+    }
+    a->jobs = 2;
+    a->direct = 0;
+    j0.spans = j1.spans = 1;
+    j0.kind[0] = kRangePrefix;
+    j1.kind[0] = kRangeOwn;
+    const int64_t pooled = rows * p->requests;
+    if (pooled * p->kv_heads > 0x7fffffffLL / 2) return unavailable("too many rows");
+    const MaskLayout y0 = mask_layout(pooled, p->kv_heads, p->prefix_tokens, cus, true);
+    const MaskLayout y1 = mask_layout(rows, groups, p->capacity, cus, true);
+    if ((rc = set_job(&j0, y0, 1, (int)p->kv_heads, pooled, 1)) != ZDRAW_HIP_OK) return rc;
+    if ((rc = set_job(&j1, y1, (int)p->requests, (int)p->kv_heads, rows, 0)) != ZDRAW_HIP_OK) return rc;
+    j1.part_base = job_rows(j0);
+    *part_rows = (size_t)(job_rows(j0) + job_rows(j1));
+    return ZDRAW_HIP_OK;
+}
+
+size_t part_bytes(size_t part_rows) { return part_rows * (kHeadDim + 2) * sizeof(float); }
+
+// What both attention calls check and set alike.
+int mask_common(uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t dtype, uint32_t causal, float scale, float softcap, uint32_t reserved) {
+    if (heads == 0 || kv_heads == 0 || head_dim == 0) return invalid("zero dimension");
+    if (heads % kv_heads != 0) return invalid("heads % kv_heads != 0");
+    if (head_dim != (uint32_t)kHeadDim) return unavailable("head_dim != 128");
+    if (heads > 65535) return unavailable("too many heads");
+    if (dtype != ZDRAW_HIP_F16 && dtype != ZDRAW_HIP_BF16) return dtype == ZDRAW_HIP_F32 ? unavailable("f32 operands") : invalid("dtype");
+    if (causal > 1) return invalid("causal");
+    if (!(scale >= 0.0f) || !std::isfinite(scale)) return invalid("scale");
+    if (!(softcap >= 0.0f) || !std::isfinite(softcap)) return invalid("softcap");
+    if (reserved != 0) return invalid("reserved");
+    return ZDRAW_HIP_OK;
+}
+
+void mask_scores(MaskArgs* a, uint32_t heads, uint32_t kv_heads, uint32_t dtype, uint32_t causal, float scale, float softcap) {
+    if (scale == 0.0f) scale = 1.0f / sqrtf((float)kHeadDim);
+    a->kv_heads = (int32_t)kv_heads;
+    a->group = (int32_t)(heads / kv_heads);
+    a->causal = (int32_t)causal;
+    a->f16 = dtype == ZDRAW_HIP_F16;
+    a->scale_log2 = 1.4426950408889634f * scale;
+    if (softcap > 0.0f) {
+        a->cap_in = 2.0f * 1.4426950408889634f * scale / softcap;
+        a->cap_out = 1.4426950408889634f * softcap;
+    }
+}
+
+int masked_shape(const ZdrawHipMaskedAttn* p) {
+    const int rc = mask_common(p->heads, p->kv_heads, p->head_dim, p->dtype, p->causal, p->scale, p->softcap, p->reserved);
+    if (rc != ZDRAW_HIP_OK) return rc;
+    if ((uint64_t)p->q_tokens * (p->heads / p->kv_heads) >= kMaskMaxTokens || p->k_tokens >= kMaskMaxTokens) return unavailable("too many tokens");
+    if ((uint64_t)p->q_tokens * p->heads * p->batch > 0x7fffffffull || p->batch > 0xffffffu) return unavailable("too many rows");
+    if (p->documents > kMaskMaxTokens) return unavailable("too many documents");
+    return ZDRAW_HIP_OK;
+}
+
+int shared_shape(const ZdrawHipSharedAttn* p) {
+    const int rc = mask_common(p->heads, p->kv_heads, p->head_dim, p->dtype, p->causal, p->scale, p->softcap, p->reserved);
+    if (rc != ZDRAW_HIP_OK) return rc;
+    if ((uint64_t)p->q_tokens * (p->heads / p->kv_heads) >= kMaskMaxTokens || (uint64_t)p->prefix_tokens + p->capacity >= kMaskMaxTokens)
+        return unavailable("too many tokens");
+    if ((uint64_t)p->q_tokens * p->heads * p->requests > 0x7fffffffull || p->requests > 0xffffffu) return unavailable("too many rows");
+    return ZDRAW_HIP_OK;
+}
+
+// Pages of a cache: power of two from 4 on, so that the four rows that one load takes lie on one page.
+int check_pages(uint32_t page_tokens, uint32_t pages, uint32_t capacity, uint32_t requests, void* table) {
+    if (page_tokens == 0) return ZDRAW_HIP_OK;
+    if ((page_tokens & (page_tokens - 1)) != 0) return invalid("page_tokens is not a power of two");
+    if (page_tokens < 4 || page_tokens > kMaskMaxTokens) return unavailable("page_tokens");
+    if (capacity == 0) return ZDRAW_HIP_OK;
+    if (pages == 0 || pages > 0x7fffffffu) return invalid("pages");
+    const uint64_t per = ((uint64_t)capacity + page_tokens - 1) / page_tokens;
+    if (!need_u32(table, per * requests)) return invalid("page_table smaller than [requests][pages of a request]");
+    return ZDRAW_HIP_OK;
+}
+
+// Room for the parts, and the launch.
+int enqueue_masked(Queue* qu, MaskArgs* a, size_t part_rows, void* workspace) {
+    if (!a->direct) {
+        const size_t ml = part_rows * 2 * sizeof(float), o = part_rows * kHeadDim * sizeof(float);
+        if (workspace) {
+            const Buffer* w = static_cast<Buffer*>(workspace);
+            if (!w->ptr || (uintptr_t)w->ptr % 16 != 0 || w->len < part_bytes(part_rows)) return invalid("workspace smaller than the call takes");
+            mark_unstable(workspace);
+            a->part_o = static_cast<float*>(w->ptr);
+            a->part_ml = a->part_o + part_rows * kHeadDim;
+        } else {
+            Buffer* bo = queue_scratch(qu, 3, o);
+            Buffer* bm = bo ? queue_scratch(qu, 4, ml) : nullptr;
+            if (!bo || !bm) {
+                set_err("scratch allocation failed");
+                return ZDRAW_HIP_ERR_HANDLE;
+            }
+            a->part_o = static_cast<float*>(bo->ptr);
+            a->part_ml = static_cast<float*>(bm->ptr);
+        }
+    }
+    const hipError_t e = launch_masked(*a, qu->stream);
+    if (e != hipSuccess) {
+        set_err("masked attention launch: %s", hipGetErrorString(e));
+        return ZDRAW_HIP_ERR_HANDLE;
+    }
+    g_dispatch += a->direct ? 1 : 2;
+    return ZDRAW_HIP_OK;
+}
+
+int span_strides(KeySpan* s, const int64_t k[3], const int64_t v[3]) {
+    s->k_ss = k[0];
+    s->k_ts = k[1];
+    s->k_hs = k[2];
+    s->v_ss = v[0];
+    s->v_ts = v[1];
+    s->v_hs = v[2];
+    if (s->k_ts >= (1ll << 28) || s->v_ts >= (1ll << 28)) return unavailable("token stride of 2^28 bytes or more");
+    return ZDRAW_HIP_OK;
+}
+
+int enqueue_attention_masked(Queue* qu, void* q, void* k, void* v, void* out, const ZdrawHipMaskedAttn* p, const ZdrawHipMaskOperands* ops) {
+    if (!p) {
+        set_err("null params");
+        return ZDRAW_HIP_ERR_HANDLE;
+    }
+    int rc = masked_shape(p);
+    if (rc != ZDRAW_HIP_OK) return rc;
+    if (p->batch == 0 || p->q_tokens == 0) return ZDRAW_HIP_OK;
+    static const ZdrawHipMaskOperands none = {nullptr, nullptr, nullptr, nullptr, nullptr};
+    if (!ops) ops = &none;
+    const uint64_t nq[3] = {p->batch, p->q_tokens, p->heads}, nk[3] = {p->batch, p->k_tokens, p->kv_heads};
+    const char* why;
+    if ((why = check_rows(q, p->q_off, p->q_stride, nq, 2, false, "q"))) return invalid(why);
+    if ((why = check_rows(out, p->out_off, p->out_stride, nq, 2, true, "out"))) return invalid(why);
+    if (p->k_tokens != 0) {
+        if ((why = check_rows(k, p->k_off, p->k_stride, nk, 2, false, "k"))) return invalid(why);
+        if ((why = check_rows(v, p->v_off, p->v_stride, nk, 2, false, "v"))) return invalid(why);
+    }
+    const uint64_t borders = ((uint64_t)p->documents + 1) * p->batch;
+    if (p->documents == 0) {
+        if (ops->q_starts || ops->k_starts) return invalid("borders without documents");
+    } else {
+        if (!need_u32(ops->q_starts, borders)) return invalid("q_starts smaller than [batch][documents + 1]");
+        if (ops->k_starts && !need_u32(ops->k_starts, borders)) return invalid("k_starts smaller than [batch][documents + 1]");
+        if (!ops->k_starts && p->q_tokens != p->k_tokens) return invalid("q_starts stand for the keys too, but q_tokens != k_tokens");
+    }
+    if (ops->prefix) {
+        if (!p->causal) return invalid("prefix without causal");
+        if (!need_u32(ops->prefix, (uint64_t)std::max(p->documents, 1u) * p->batch)) return invalid("prefix smaller than [batch][documents]");
+    }
+    if (ops->slopes && !need_u32(ops->slopes, p->heads)) return invalid("slopes smaller than f32 [heads]");
+
+    MaskArgs a;
+    memset(&a, 0, sizeof(a));
+    int64_t qs[3], os[3], ks[3], vs[3];
+    byte_strides(qs, p->q_stride, nq, 2);
+    byte_strides(os, p->out_stride, nq, 2);
+    byte_strides(ks, p->k_stride, nk, 2);
+    byte_strides(vs, p->v_stride, nk, 2);
+    a.q = static_cast<const char*>(at(static_cast<Buffer*>(q), p->q_off));
+    a.o = const_cast<char*>(static_cast<const char*>(at(static_cast<Buffer*>(out), p->out_off)));
+    a.q_ss = qs[0]; a.q_ts = qs[1]; a.q_hs = qs[2];
+    a.o_ss = os[0]; a.o_ts = os[1]; a.o_hs = os[2];
+    a.q_starts = u32_of(ops->q_starts);
+    a.k_starts = ops->k_starts ? u32_of(ops->k_starts) : a.q_starts;
+    a.prefix = u32_of(ops->prefix);
+    a.slopes = f32_of(ops->slopes);
+    a.documents = (int32_t)p->documents;
+    a.q_tokens = (int32_t)p->q_tokens;
+    mask_scores(&a, p->heads, p->kv_heads, p->dtype, p->causal, p->scale, p->softcap);
+    KeySpan& sp = a.job[0].span[0];
+    if (p->k_tokens != 0) {
+        sp.k = static_cast<const char*>(at(static_cast<Buffer*>(k), p->k_off));
+        sp.v = static_cast<const char*>(at(static_cast<Buffer*>(v), p->v_off));
+        if ((rc = span_strides(&sp, ks, vs)) != ZDRAW_HIP_OK) return rc;
+        sp.keys = (int32_t)p->k_tokens;
+    }
+    size_t part_rows = 0;
+    rc = plan_masked_jobs(p, qu->dev->cus, ops->workspace != nullptr || !capturing(qu), &a, &part_rows);
+    if (rc != ZDRAW_HIP_OK) return rc;
+    mark_unstable(out);
+    return enqueue_masked(qu, &a, part_rows, ops->workspace);
+}
+
+int enqueue_attention_shared(Queue* qu, void* q, void* prefix_k, void* prefix_v, void* k, void* v, void* out, const ZdrawHipSharedAttn* p,
+                             const ZdrawHipSharedOperands* ops) {
+    if (!p || !ops) {
+        set_err("null params");
+        return ZDRAW_HIP_ERR_HANDLE;
+    }
+    int rc = shared_shape(p);
+    if (rc != ZDRAW_HIP_OK) return rc;
+    if (p->requests == 0 || p->q_tokens == 0) return ZDRAW_HIP_OK;
+    const bool paged = p->page_tokens != 0;
+    if ((rc = check_pages(p->page_tokens, p->pages, p->capacity, p->requests, ops->page_table)) != ZDRAW_HIP_OK) return rc;
+    if (!paged && ops->page_table) return invalid("page_table without page_tokens");
+    const uint64_t nq[3] = {p->requests, p->q_tokens, p->heads}, np[3] = {1, p->prefix_tokens, p->kv_heads};
+    const uint64_t nk[3] = {paged ? p->pages : p->requests, paged ? p->page_tokens : p->capacity, p->kv_heads};
+    const uint64_t pks[3] = {0, p->prefix_k_stride[0], p->prefix_k_stride[1]}, pvs[3] = {0, p->prefix_v_stride[0], p->prefix_v_stride[1]};
+    const char* why;
+    if ((why = check_rows(q, p->q_off, p->q_stride, nq, 2, false, "q"))) return invalid(why);
+    if ((why = check_rows(out, p->out_off, p->out_stride, nq, 2, true, "out"))) return invalid(why);
+    if (p->prefix_tokens != 0) {
+        if ((why = check_rows(prefix_k, p->prefix_k_off, pks, np, 2, false, "prefix_k"))) return invalid(why);
+        if ((why = check_rows(prefix_v, p->prefix_v_off, pvs, np, 2, false, "prefix_v"))) return invalid(why);
+    }
+    if (p->capacity != 0) {
+        if ((why = check_rows(k, p->k_off, p->k_stride, nk, 2, false, "k"))) return invalid(why);
+        if ((why = check_rows(v, p->v_off, p->v_stride, nk, 2, false, "v"))) return invalid(why);
+        if (!need_u32(ops->lens, p->requests)) return invalid("lens smaller than [requests]");
+    }
+    if (ops->q_lens && !need_u32(ops->q_lens, p->requests)) return invalid("q_lens smaller than [requests]");
+    if (ops->slopes && !need_u32(ops->slopes, p->heads)) return invalid("slopes smaller than f32 [heads]");
+
+    MaskArgs a;
+    memset(&a, 0, sizeof(a));
+    int64_t qs[3], os[3], ks[3], vs[3];
+    byte_strides(qs, p->q_stride, nq, 2);
+    byte_strides(os, p->out_stride, nq, 2);
+    a.q = static_cast<const char*>(at(static_cast<Buffer*>(q), p->q_off));
+    a.o = const_cast<char*>(static_cast<const char*>(at(static_cast<Buffer*>(out), p->out_off)));
+    a.q_ss = qs[0]; a.q_ts = qs[1]; a.q_hs = qs[2];
+    a.o_ss = os[0]; a.o_ts = os[1]; a.o_hs = os[2];
+    a.lens = p->capacity != 0 ? u32_of(ops->lens) : nullptr;
+    a.q_lens = u32_of(ops->q_lens);
+    a.slopes = f32_of(ops->slopes);
+    a.q_tokens = (int32_t)p->q_tokens;
+    a.own_keys = (int32_t)p->capacity;
+    mask_scores(&a, p->heads, p->kv_heads, p->dtype, p->causal, p->scale, p->softcap);
+    size_t part_rows = 0;
+    rc = plan_shared_jobs(p, qu->dev->cus, ops->workspace != nullptr || !capturing(qu), &a, &part_rows);
+    if (rc != ZDRAW_HIP_OK) return rc;
+    KeySpan prefix, mine;
+    memset(&prefix, 0, sizeof(prefix));
+    memset(&mine, 0, sizeof(mine));
+    if (p->prefix_tokens != 0) {
+        byte_strides(ks, pks, np, 2);
+        byte_strides(vs, pvs, np, 2);
+        prefix.k = static_cast<const char*>(at(static_cast<Buffer*>(prefix_k), p->prefix_k_off));
+        prefix.v = static_cast<const char*>(at(static_cast<Buffer*>(prefix_v), p->prefix_v_off));
+        if ((rc = span_strides(&prefix, ks, vs)) != ZDRAW_HIP_OK) return rc;
+        prefix.keys = (int32_t)p->prefix_tokens;
+    }
+    if (p->capacity != 0) {
+        byte_strides(ks, p->k_stride, nk, 2);
+        byte_strides(vs, p->v_stride, nk, 2);
+        mine.k = static_cast<const char*>(at(static_cast<Buffer*>(k), p->k_off));
+        mine.v = static_cast<const char*>(at(static_cast<Buffer*>(v), p->v_off));
+        if ((rc = span_strides(&mine, ks, vs)) != ZDRAW_HIP_OK) return rc;
+        mine.keys = (int32_t)p->capacity;
+        if (paged) {
+            mine.table = u32_of(ops->page_table);
+            mine.table_ld = (int32_t)((p->capacity + p->page_tokens - 1) / p->page_tokens);
+            mine.page_shift = __builtin_ctz(p->page_tokens);
+            mine.page_mask = (int32_t)p->page_tokens - 1;
+            mine.pages = (int32_t)p->pages;
+        }
+    }
+    for (int i = 0; i < a.jobs; i++)
+        for (int s = 0; s < a.job[i].spans; s++) a.job[i].span[s] = a.job[i].kind[s] == kRangePrefix ? prefix : mine;
+    mark_unstable(out);
+    return enqueue_masked(qu, &a, part_rows, ops->workspace);
+}
+
+int enqueue_kv_append(Queue* qu, void* q, void* k, void* v, void* q_out, void* cache_k, void* cache_v, const ZdrawHipKvAppend* p,
+                      const ZdrawHipAppendOperands* ops) {
+    if (!p || !ops) {
+        set_err("null params");
+        return ZDRAW_HIP_ERR_HANDLE;
+    }
+    if (p->kv_heads == 0 || p->head_dim == 0) return invalid("zero dimension");
+    if (p->head_dim != (uint32_t)kHeadDim) return unavailable("head_dim != 128");
+    if (p->heads > 65535 || p->kv_heads > 65535) return unavailable("too many heads");
+    if (p->in_dtype > ZDRAW_HIP_BF16 || (p->dtype != ZDRAW_HIP_F16 && p->dtype != ZDRAW_HIP_BF16)) return p->dtype == ZDRAW_HIP_F32 ? unavailable("f32 cache") : invalid("dtype");
+    if (p->rotation > ZDRAW_HIP_ROTATE_HALVES) return invalid("rotation");
+    if (!(p->eps >= 0.0f) || !std::isfinite(p->eps)) return invalid("eps");
+    if (p->capacity >= kMaskMaxTokens || p->tokens >= kMaskMaxTokens || p->requests > 0xffffffu) return unavailable("too many tokens");
+    const uint64_t slots = (uint64_t)p->heads + 2 * (uint64_t)p->kv_heads;
+    if ((unsigned __int128)p->requests * p->tokens * slots > 0x7fffffffu) return unavailable("too many rows");
+    if (p->requests == 0 || p->tokens == 0) return ZDRAW_HIP_OK;
+    if (p->capacity == 0) return invalid("capacity == 0");
+    int rc;
+    const bool paged = p->page_tokens != 0;
+    if ((rc = check_pages(p->page_tokens, p->pages, p->capacity, p->requests, ops->page_table)) != ZDRAW_HIP_OK) return rc;
+    if (!paged && ops->page_table) return invalid("page_table without page_tokens");
+    const size_t es = elem_size(p->in_dtype);
+    const uint64_t nq[3] = {p->requests, p->tokens, p->heads}, nk[3] = {p->requests, p->tokens, p->kv_heads};
+    const uint64_t nc[3] = {paged ? p->pages : p->requests, paged ? p->page_tokens : p->capacity, p->kv_heads};
+    const char* why;
+    if (p->heads != 0) {
+        if ((why = check_rows(q, p->q_off, p->q_stride, nq, es, false, "q"))) return invalid(why);
+        if ((why = check_rows(q_out, p->q_out_off, p->q_out_stride, nq, 2, true, "q_out"))) return invalid(why);
+    } else if (ops->q_weight) {
+        return invalid("q_weight without query heads");
+    }
+    if ((why = check_rows(k, p->k_off, p->k_stride, nk, es, false, "k"))) return invalid(why);
+    if ((why = check_rows(v, p->v_off, p->v_stride, nk, es, false, "v"))) return invalid(why);
+    if ((why = check_rows(cache_k, p->cache_k_off, p->cache_k_stride, nc, 2, true, "cache_k"))) return invalid(why);
+    if ((why = check_rows(cache_v, p->cache_v_off, p->cache_v_stride, nc, 2, true, "cache_v"))) return invalid(why);
+    if (!need_u32(ops->starts, p->requests)) return invalid("starts smaller than [requests]");
+    if (ops->counts && !need_u32(ops->counts, p->requests)) return invalid("counts smaller than [requests]");
+    if ((ops->q_weight && !need(ops->q_weight, kHeadDim * 4)) || (ops->k_weight && !need(ops->k_weight, kHeadDim * 4)))
+        return invalid("norm weights must be f32[128] buffers");
+    if (p->rotation != ZDRAW_HIP_ROTATE_NONE) {
+        const size_t bytes = (size_t)p->rope_rows * kHeadDim * 4;
+        if (p->rope_rows == 0 || !need(ops->rope_cos, bytes) || !need(ops->rope_sin, bytes)) return invalid("rope cos/sin tables too small for [rope_rows][128] f32");
+    }
+
+    AppendArgs a;
+    memset(&a, 0, sizeof(a));
+    if (p->heads != 0) {
+        a.q = static_cast<const char*>(at(static_cast<Buffer*>(q), p->q_off));
+        a.qo = const_cast<char*>(static_cast<const char*>(at(static_cast<Buffer*>(q_out), p->q_out_off)));
+        byte_strides(a.q_s, p->q_stride, nq, es);
+        byte_strides(a.qo_s, p->q_out_stride, nq, 2);
+        mark_unstable(q_out);
+    }
+    a.k = static_cast<const char*>(at(static_cast<Buffer*>(k), p->k_off));
+    a.v = static_cast<const char*>(at(static_cast<Buffer*>(v), p->v_off));
+    a.ck = const_cast<char*>(static_cast<const char*>(at(static_cast<Buffer*>(cache_k), p->cache_k_off)));
+    a.cv = const_cast<char*>(static_cast<const char*>(at(static_cast<Buffer*>(cache_v), p->cache_v_off)));
+    byte_strides(a.k_s, p->k_stride, nk, es);
+    byte_strides(a.v_s, p->v_stride, nk, es);
+    byte_strides(a.ck_s, p->cache_k_stride, nc, 2);
+    byte_strides(a.cv_s, p->cache_v_stride, nc, 2);
+    mark_unstable(cache_k);
+    mark_unstable(cache_v);
+    a.starts = u32_of(ops->starts);
+    a.counts = u32_of(ops->counts);
+    if (paged) {
+        a.table = u32_of(ops->page_table);
+        a.table_ld = (int32_t)((p->capacity + p->page_tokens - 1) / p->page_tokens);
+        a.page_shift = __builtin_ctz(p->page_tokens);
+        a.page_mask = (int32_t)p->page_tokens - 1;
+        a.pages = (int32_t)p->pages;
+    }
+    a.q_w = f32_of(ops->q_weight);
+    a.k_w = f32_of(ops->k_weight);
+    a.cos_t = f32_of(ops->rope_cos);
+    a.sin_t = f32_of(ops->rope_sin);
+    a.requests = (int32_t)p->requests;
+    a.tokens = (int32_t)p->tokens;
+    a.capacity = (int32_t)p->capacity;
+    a.heads = (int32_t)p->heads;
+    a.kv_heads = (int32_t)p->kv_heads;
+    a.rotation = (int32_t)p->rotation;
+    a.rope_rows = (int32_t)std::min(p->rope_rows, 0x7fffffffu);
+    a.position_base = p->position_base;
+    a.in_dtype = (int32_t)p->in_dtype;
+    a.dtype = (int32_t)p->dtype;
+    a.eps = p->eps;
+    const hipError_t e = launch_kv_append(a, qu->stream);
+    if (e != hipSuccess) {
+        set_err("cache append launch: %s", hipGetErrorString(e));
+        return ZDRAW_HIP_ERR_HANDLE;
+    }
+    g_dispatch++;
+    return ZDRAW_HIP_OK;
+}
+
+// The blocking form of an entry that takes a batch.
+template <typename Enqueue>
+int run_blocking(void* queue, Enqueue enqueue_on) {
+    void* b = zdraw_hip_batch_begin(queue);
+    if (!b) {
+        set_err("null queue");
+        return ZDRAW_HIP_ERR_HANDLE;
+    }
+    const int rc = enqueue_on(static_cast<Batch*>(b)->queue);
+    const int rc2 = zdraw_hip_batch_end(b);
+    return rc != ZDRAW_HIP_OK ? rc : rc2;
+}
+
+template <typename Enqueue>
+int run_on_batch(void* batch, Enqueue enqueue_on) {
+    if (!batch) {
+        set_err("null batch");
+        return ZDRAW_HIP_ERR_HANDLE;
+    }
+    return enqueue_on(static_cast<Batch*>(batch)->queue);
+}
+
+} // namespace
+
+extern "C" {
+
+int zdraw_hip_run_attention_masked_enc(void* batch, void* q, void* k, void* v, void* out, const ZdrawHipMaskedAttn* params,
+                                       const ZdrawHipMaskOperands* ops) {
+    return run_on_batch(batch, [&](Queue* qu) { return enqueue_attention_masked(qu, q, k, v, out, params, ops); });
+}
+
+int zdraw_hip_run_attention_masked(void* queue, void* q, void* k, void* v, void* out, const ZdrawHipMaskedAttn* params,
+                                   const ZdrawHipMaskOperands* ops) {
+    return run_blocking(queue, [&](Queue* qu) { return enqueue_attention_masked(qu, q, k, v, out, params, ops); });
+}
+
+size_t zdraw_hip_attention_masked_workspace(void* queue, const ZdrawHipMaskedAttn* params) {
+    const Queue* qu = static_cast<Queue*>(queue);
+    if (!qu || !params || masked_shape(params) != ZDRAW_HIP_OK || params->batch == 0 || params->q_tokens == 0) return 0;
+    MaskArgs a;
+    memset(&a, 0, sizeof(a));
+    size_t rows = 0;
+    return plan_masked_jobs(params, qu->dev->cus, true, &a, &rows) == ZDRAW_HIP_OK ? part_bytes(rows) : 0;
+}
+
+int zdraw_hip_run_attention_shared_enc(void* batch, void* q, void* prefix_k, void* prefix_v, void* k, void* v, void* out,
+                                       const ZdrawHipSharedAttn* params, const ZdrawHipSharedOperands* ops) {
+    return run_on_batch(batch, [&](Queue* qu) { return enqueue_attention_shared(qu, q, prefix_k, prefix_v, k, v, out, params, ops); });
+}
+
+int zdraw_hip_run_attention_shared(void* queue, void* q, void* prefix_k, void* prefix_v, void* k, void* v, void* out,
+                                   const ZdrawHipSharedAttn* params, const ZdrawHipSharedOperands* ops) {
+    return run_blocking(queue, [&](Queue* qu) { return enqueue_attention_shared(qu, q, prefix_k, prefix_v, k, v, out, params, ops); });
+}
+
+size_t zdraw_hip_attention_shared_workspace(void* queue, const ZdrawHipSharedAttn* params) {
+    const Queue* qu = static_cast<Queue*>(queue);
+    if (!qu || !params || shared_shape(params) != ZDRAW_HIP_OK || params->requests == 0 || params->q_tokens == 0) return 0;
+    MaskArgs a;
+    memset(&a, 0, sizeof(a));
+    size_t rows = 0;
+    return plan_shared_jobs(params, qu->dev->cus, true, &a, &rows) == ZDRAW_HIP_OK ? part_bytes(rows) : 0;
+}
+
+int zdraw_hip_run_kv_append_enc(void* batch, void* q, void* k, void* v, void* q_out, void* cache_k, void* cache_v,
+                                const ZdrawHipKvAppend* params, const ZdrawHipAppendOperands* ops) {
+    return run_on_batch(batch, [&](Queue* qu) { return enqueue_kv_append(qu, q, k, v, q_out, cache_k, cache_v, params, ops); });
+}
+
+int zdraw_hip_run_kv_append(void* queue, void* q, void* k, void* v, void* q_out, void* cache_k, void* cache_v,
+                            const ZdrawHipKvAppend* params, const ZdrawHipAppendOperands* ops) {
+    return run_blocking(queue, [&](Queue* qu) { return enqueue_kv_append(qu, q, k, v, q_out, cache_k, cache_v, params, ops); });
+}
+
 // ------------------------------------------------------------------ scratch
 void* zdraw_hip_attn_scratch(void* device, int slot, size_t bytes) {
     if (!device || slot < 0 || slot >= kCallerSlots || bytes == 0) return nullptr;
@@ -2063,6 +2612,12 @@ size_t zdraw_hip_abi_sizeof(int which) {
     case 6: return sizeof(ZdrawHipChainAttnBuffers);
     case 7: return sizeof(ZdrawHipChainAttnWeights);
     case 8: return sizeof(ZdrawHipChainAttnParams);
+    case 9: return sizeof(ZdrawHipMaskedAttn);
+    case 10: return sizeof(ZdrawHipMaskOperands);
+    case 11: return sizeof(ZdrawHipSharedAttn);
+    case 12: return sizeof(ZdrawHipSharedOperands);
+    case 13: return sizeof(ZdrawHipKvAppend);
+    case 14: return sizeof(ZdrawHipAppendOperands);
     default: return 0;
     }
 }

@@ -1,0 +1,97 @@
+// Internal launch interface of the attention over row ranges (attn_masked.hip) and of the cache append
+// (kv_append.hip). Not part of the public ABI (that is include/zdraw_hip.h).
+#pragma once
+
+#include "attn_kernel.h"
+
+namespace zdraw {
+
+// Where a sequence's keys and values lie: rows of 128 16-bit elements, strides in bytes. With a page table, key j of
+// sequence s is row j & page_mask of page table[s * table_ld + (j >> page_shift)] and k_ss / v_ss are between pages.
+struct KeySpan {
+    const char* k;
+    const char* v;
+    int64_t k_ss, k_hs, v_ss, v_hs; // between sequences (or pages), between key heads
+    int64_t k_ts, v_ts;             // between tokens; below 2^28
+    const unsigned* table;          // null: no pages
+    int32_t table_ld, page_shift, page_mask, pages;
+    int32_t keys;                   // the most keys of a sequence
+};
+
+enum RangeKind : int {
+    kRangeDocs = 0,   // rows of packed documents (or of one): MaskArgs q_starts, k_starts, prefix
+    kRangePrefix = 1, // every row sees all keys
+    kRangeOwn = 2,    // a request's own keys: lens, q_lens
+};
+
+// A set of workgroups: every (sequence, key head, tile of rows, share of the keys) is one. Rows are (token, query head
+// of the key head's group), tokens outermost.
+struct MaskJob {
+    KeySpan span[2];
+    int32_t kind[2];
+    int32_t spans;     // 1, or 2: walked one after the other
+    int32_t by_keys;   // 0: 128 rows, 32 per wave, all waves share every key block; 1: 32 rows, the waves take key blocks in turn
+    int32_t seqs;      // sequences whose rows are tiled by themselves
+    int32_t pooled;    // 1: the rows of all sequences are one row space (seqs == 1)
+    int32_t rows;      // per sequence
+    int32_t row_tiles, splits;
+    int32_t workgroups; // seqs * kv_heads * row_tiles * splits
+    int64_t part_base; // first row of this job's parts in part_o / part_ml
+};
+
+struct MaskArgs {
+    const char* q;
+    char* o;
+    int64_t q_ss, q_ts, q_hs, o_ss, o_ts, o_hs; // bytes: between sequences, tokens, heads
+    const unsigned* q_starts; // documents: borders [seq][documents + 1], or null
+    const unsigned* k_starts;
+    const unsigned* prefix;   // [seq][documents], or null
+    const unsigned* lens;     // requests' own keys
+    const unsigned* q_lens;   // or null
+    const float* slopes;      // [heads], or null
+    int32_t documents, q_tokens, causal;
+    int32_t own_keys;         // room for a request's own keys
+    int32_t kv_heads, group;
+    float scale_log2;         // log2(e) * scale
+    float cap_in, cap_out;    // 2 log2(e) scale / cap, log2(e) cap; cap_in == 0: scores are not capped
+    int32_t f16;
+    int32_t jobs;
+    MaskJob job[2];
+    float* part_o;  // [row][128] unnormalised
+    float* part_ml; // [row][2]: reference point (log2), denominator
+    int32_t direct; // 1: one job without splits, which writes the output itself
+};
+
+constexpr int kMaskRowsByWave = 128; // rows of a workgroup whose waves share key blocks
+constexpr int kMaskRowsByKeys = 32;
+
+hipError_t masked_setup();
+hipError_t launch_masked(const MaskArgs& a, hipStream_t stream);
+
+struct AppendArgs {
+    const char* q; // null: no query rows
+    const char* k;
+    const char* v;
+    char* qo;
+    char* ck;
+    char* cv;
+    // bytes: [0] between requests (pages), [1] between tokens, [2] between heads
+    int64_t q_s[3], k_s[3], v_s[3], qo_s[3], ck_s[3], cv_s[3];
+    const unsigned* starts;
+    const unsigned* counts; // or null: all of them
+    const unsigned* table;  // or null
+    const float* q_w;       // or null: no norm
+    const float* k_w;
+    const float* cos_t;
+    const float* sin_t;
+    int32_t table_ld, page_shift, page_mask, pages;
+    int32_t requests, tokens, capacity, heads, kv_heads;
+    int32_t rotation; // 0 none, 1 adjacent pairs, 2 halves
+    int32_t rope_rows;
+    uint32_t position_base;
+    int32_t in_dtype, dtype;
+    float eps;
+};
+hipError_t launch_kv_append(const AppendArgs& a, hipStream_t stream);
+
+} // namespace zdraw

@@ -80,8 +80,50 @@ class ChainAttnParams(C.Structure):
                 ("attn", AttnParams), ("proj", GemmParams), ("act_dtype", C.c_uint32), ("score_bound", C.c_float)]
 
 
+class MaskedAttn(C.Structure):
+    """ZdrawHipMaskedAttn"""
+    _fields_ = [("q_off", C.c_uint64), ("k_off", C.c_uint64), ("v_off", C.c_uint64), ("out_off", C.c_uint64),
+                ("q_stride", C.c_uint64 * 3), ("k_stride", C.c_uint64 * 3), ("v_stride", C.c_uint64 * 3), ("out_stride", C.c_uint64 * 3),
+                ("batch", C.c_uint32), ("q_tokens", C.c_uint32), ("k_tokens", C.c_uint32), ("heads", C.c_uint32), ("kv_heads", C.c_uint32),
+                ("head_dim", C.c_uint32), ("dtype", C.c_uint32), ("causal", C.c_uint32), ("documents", C.c_uint32),
+                ("scale", C.c_float), ("softcap", C.c_float), ("reserved", C.c_uint32)]
+
+
+class MaskOperands(C.Structure):
+    """ZdrawHipMaskOperands"""
+    _fields_ = [(n, C.c_void_p) for n in ("q_starts", "k_starts", "prefix", "slopes", "workspace")]
+
+
+class SharedAttn(C.Structure):
+    """ZdrawHipSharedAttn"""
+    _fields_ = [(n, C.c_uint64) for n in ("q_off", "out_off", "prefix_k_off", "prefix_v_off", "k_off", "v_off")] + [
+        ("q_stride", C.c_uint64 * 3), ("out_stride", C.c_uint64 * 3), ("prefix_k_stride", C.c_uint64 * 2), ("prefix_v_stride", C.c_uint64 * 2),
+        ("k_stride", C.c_uint64 * 3), ("v_stride", C.c_uint64 * 3)] + [(n, C.c_uint32) for n in (
+            "requests", "q_tokens", "prefix_tokens", "capacity", "page_tokens", "pages", "heads", "kv_heads", "head_dim", "dtype", "causal")] + [
+        ("scale", C.c_float), ("softcap", C.c_float), ("reserved", C.c_uint32)]
+
+
+class SharedOperands(C.Structure):
+    """ZdrawHipSharedOperands"""
+    _fields_ = [(n, C.c_void_p) for n in ("lens", "q_lens", "page_table", "slopes", "workspace")]
+
+
+class KvAppend(C.Structure):
+    """ZdrawHipKvAppend"""
+    _fields_ = [(n, C.c_uint64) for n in ("q_off", "k_off", "v_off", "q_out_off", "cache_k_off", "cache_v_off")] + [
+        (n, C.c_uint64 * 3) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride", "cache_k_stride", "cache_v_stride")] + [
+        (n, C.c_uint32) for n in ("requests", "tokens", "capacity", "page_tokens", "pages", "heads", "kv_heads", "head_dim", "in_dtype", "dtype",
+                                  "rotation", "rope_rows", "position_base")] + [("eps", C.c_float)]
+
+
+class AppendOperands(C.Structure):
+    """ZdrawHipAppendOperands"""
+    _fields_ = [(n, C.c_void_p) for n in ("starts", "counts", "page_table", "q_weight", "k_weight", "rope_cos", "rope_sin")]
+
+
 W_F16, W_BF16, W_F32 = 1, 2, 3     # weight dtype codes of GemmParams.dtype
 GEMM_EXACT, GEMM_HALF = 1, 2       # GemmParams.mode
+ROTATE_NONE, ROTATE_PAIRS, ROTATE_HALVES = 0, 1, 2  # KvAppend.rotation
 
 # every symbol include/*.h declares: name -> (restype, argtypes)
 _vp, _sz, _u32, _u64, _int = C.c_void_p, C.c_size_t, C.c_uint32, C.c_uint64, C.c_int
@@ -137,6 +179,14 @@ SYMBOLS = {
     "zdraw_hip_run_gemm_group_ext_enc": (_int, [_vp, _vp, C.POINTER(_vp), C.POINTER(_vp), C.POINTER(_GP), C.c_uint32, _GX]),
     "zdraw_hip_run_chain_attn_enc": (_int, [_vp, C.POINTER(ChainAttnBuffers), C.POINTER(ChainAttnWeights),
                                             C.POINTER(ChainAttnParams)]),
+    "zdraw_hip_run_attention_masked_enc": (_int, [_vp] * 5 + [C.POINTER(MaskedAttn), C.POINTER(MaskOperands)]),
+    "zdraw_hip_run_attention_masked": (_int, [_vp] * 5 + [C.POINTER(MaskedAttn), C.POINTER(MaskOperands)]),
+    "zdraw_hip_attention_masked_workspace": (_sz, [_vp, C.POINTER(MaskedAttn)]),
+    "zdraw_hip_run_attention_shared_enc": (_int, [_vp] * 7 + [C.POINTER(SharedAttn), C.POINTER(SharedOperands)]),
+    "zdraw_hip_run_attention_shared": (_int, [_vp] * 7 + [C.POINTER(SharedAttn), C.POINTER(SharedOperands)]),
+    "zdraw_hip_attention_shared_workspace": (_sz, [_vp, C.POINTER(SharedAttn)]),
+    "zdraw_hip_run_kv_append_enc": (_int, [_vp] * 7 + [C.POINTER(KvAppend), C.POINTER(AppendOperands)]),
+    "zdraw_hip_run_kv_append": (_int, [_vp] * 7 + [C.POINTER(KvAppend), C.POINTER(AppendOperands)]),
     "zdraw_hip_clock_probe": (None, [_int]),
     "zdraw_hip_clock_probe_read": (C.c_size_t, [C.POINTER(C.c_uint64), C.POINTER(C.c_uint64), C.c_size_t]),
     "zdraw_hip_event_create": (_vp, []),
