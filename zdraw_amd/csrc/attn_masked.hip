@@ -29,7 +29,8 @@ constexpr int kRow = D * 2;           // bytes of a row
 constexpr int kBlock = KB * kRow;     // bytes of a K (or V) block
 constexpr int kStages = 4;
 constexpr int kLds = kStages * 2 * kBlock;
-constexpr float kTau = 8.0f; // a row's reference point moves when a score (log2) lies this far above it: P <= 2^8 fits IEEE half
+constexpr float kTau = 8.0f;     // a row's reference point moves when a score (log2) lies this far above it: P <= 2^8 fits IEEE half
+constexpr float kLimit = 256.0f; // or when a lane's 16 of a block add up to more
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -42,6 +43,12 @@ __device__ __forceinline__ float lane_f(float x, int src) { return __uint_as_flo
 // 1 KB of one operand, four rows of 256 bytes, to LDS: lane i's 16 bytes land at lds + 16 i.
 __device__ __forceinline__ void rows_to_lds(const char* base, unsigned lane_off, unsigned lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(lane_off), "s"(base) : "memory", "m0");
+}
+
+// Keeps what forms a value on this side of the point where it is called.
+template <typename T>
+__device__ __forceinline__ void pin(T& v) {
+    asm volatile("" : "+v"(v));
 }
 
 template <int N>
@@ -165,22 +172,26 @@ __device__ __forceinline__ void row_at(const KeySpan& sp, const SpanBase& b, int
     }
 }
 
-// Lane offsets of a four-row load: row lane / 16 of the four, chunk by the swizzle of LDS row 4 n + lane / 16.
-struct LoadLane {
-    unsigned q;          // lane / 16
-    unsigned kc[4], vc;  // byte offset of the chunk in its row
-    unsigned k_ts, v_ts;
-};
+// The lane's number formed anew, so that what is made from it in a seldom taken branch holds no register outside of it.
+__device__ __forceinline__ int lane_again() {
+    int x;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(x));
+    return x;
+}
 
-// Loads rows j .. j + 3 of K and V (n = the first one's place in the block / 4); rows past `last` repeat it.
-template <bool K, bool V>
-__device__ __forceinline__ void load_rows(const KeySpan& sp, const SpanBase& b, const LoadLane& ln, int j, int last, int n, unsigned k_lds, unsigned v_lds) {
+// A load takes four rows: lane i the 16-byte chunk of row i / 16 that the swizzle places at chunk i % 16 of LDS row 4 n + i / 16.
+__device__ __forceinline__ unsigned k_chunk(int lane, int n) { return (((unsigned)lane & 15u) ^ ((4u * (unsigned)n + ((unsigned)lane >> 4)) & 15u)) * 16u; }
+__device__ __forceinline__ unsigned v_chunk(int lane) { return (((unsigned)lane & 15u) ^ (((unsigned)lane >> 4) << 2)) * 16u; }
+
+// Loads rows j .. j + 3 of K or V (n = the first one's place in the block / 4); rows past `last` repeat it.
+template <bool V>
+__device__ __forceinline__ void load_rows(const KeySpan& sp, const SpanBase& b, int lane, int j, int last, int n, unsigned lds) {
     const char *kp, *vp;
     row_at(sp, b, min(j, last), kp, vp);
-    unsigned q = ln.q;
+    unsigned q = (unsigned)lane >> 4;
     if (j + 3 > last) q = min(q, (unsigned)max(last - j, 0));
-    if (K) rows_to_lds(kp, q * ln.k_ts + ln.kc[n & 3], k_lds + (unsigned)n * 1024u);
-    if (V) rows_to_lds(vp, q * ln.v_ts + ln.vc, v_lds + (unsigned)n * 1024u);
+    if (V) rows_to_lds(vp, q * (unsigned)sp.v_ts + v_chunk(lane), lds + (unsigned)n * 1024u);
+    else rows_to_lds(kp, q * (unsigned)sp.k_ts + k_chunk(lane, n), lds + (unsigned)n * 1024u);
 }
 
 // What a lane keeps of its row across the key blocks. O^T: lane row l32, dims 32 b + 8 i + 4 h + j in o[b][4 i + j].
@@ -195,8 +206,8 @@ __device__ __forceinline__ f32x16 mfma(const bf16x8& x, const bf16x8& y, const f
     else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0);
 }
 
-template <bool F16>
-__device__ __forceinline__ bf16x8 round8(const f32x16& p, int at) {
+template <bool F16, typename T>
+__device__ __forceinline__ bf16x8 round8(const T& p, int at) {
     f32x8 x;
 #pragma unroll
     for (int i = 0; i < 8; i++) x[i] = p[at + i];
@@ -204,39 +215,42 @@ __device__ __forceinline__ bf16x8 round8(const f32x16& p, int at) {
     else return __builtin_convertvector(x, bf16x8);
 }
 
-// A score of one key, log2, from the product q.k (cap and bias; the plain scale is applied by the caller's fma).
-__device__ __forceinline__ float fancy_score(const MaskArgs& a, float dot, float slope, float dist) {
-    float y;
-    if (a.cap_in != 0.0f) {
-        // cap tanh(s / cap): tanh x = 1 - 2 / (e^2x + 1) is 1 and -1 at the infinities and NaN at NaN; near 0 it is off by 2^-24 of the cap
-        y = a.cap_out * (1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(dot * a.cap_in) + 1.0f));
-    } else {
-        y = dot * a.scale_log2;
-    }
-    return y - slope * fabsf(dist);
-}
+// What becomes of a product q.k before the softmax.
+enum ScoreMode : int { kPlain = 0, kBias = 1, kCap = 2 }; // kCap: and biased, by a slope that may be 0
 
-// Scores of a block -> P (16 bits), with the row's reference point, denominator and O kept up. `whole`: every row of the
-// wave sees the whole block.
-template <bool F16, bool FANCY>
-__device__ __forceinline__ void softmax_block(const MaskArgs& a, f32x16& s, int j0, int h, const Range& r, float slope, bool whole, RowState& st, bf16x8 (&p)[2]) {
-    float c = a.scale_log2;
-    if constexpr (FANCY) {
-        const float d0 = (float)(r.pos - j0 - 4 * h);
+// A score of one key, log2, where it is more than a scaled product (kPlain: the scale is in the exponential's fma).
+template <int MODE>
+__device__ __forceinline__ float score_of(const MaskArgs& a, float dot, float slope, float dist) {
+    // cap tanh(s / cap): tanh x = 1 - 2 / (e^2x + 1) is 1 and -1 at the infinities and NaN at NaN; near 0 it is off by 2^-24 of the cap
+    const float y = MODE == kCap ? __builtin_fmaf(-2.0f * a.cap_out, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(dot * a.cap_in) + 1.0f), a.cap_out) : dot * a.scale_log2;
+    return __builtin_fmaf(-slope, fabsf(dist), y);
+}
+template <int MODE>
+__device__ __forceinline__ void score_block(const MaskArgs& a, f32x16& s, int j0, int h, int pos, float slope) {
+    if constexpr (MODE != kPlain) {
+        const float d0 = (float)(pos - j0 - 4 * h);
 #pragma unroll
-        for (int i = 0; i < 16; i++) s[i] = fancy_score(a, s[i], slope, d0 - (float)(8 * (i >> 2) + (i & 3)));
-        c = 1.0f;
+        for (int i = 0; i < 16; i++) s[i] = score_of<MODE>(a, s[i], slope, d0 - (float)(8 * (i >> 2) + (i & 3)));
     }
-    if (!whole) {
-        const unsigned n = (unsigned)(r.hi - r.lo);
-        const unsigned first = (unsigned)(j0 + 4 * h - r.lo);
+}
+__device__ __forceinline__ void mask_block(f32x16& s, int j0, int h, const Range& r) {
+    const unsigned n = (unsigned)(r.hi - r.lo);
+    const unsigned first = (unsigned)(j0 + 4 * h - r.lo);
 #pragma unroll
-        for (int i = 0; i < 16; i++) s[i] = first + (unsigned)(8 * (i >> 2) + (i & 3)) < n ? s[i] : -INFINITY;
-    }
+    for (int i = 0; i < 16; i++) s[i] = first + (unsigned)(8 * (i >> 2) + (i & 3)) < n ? s[i] : -INFINITY;
+}
+__device__ __forceinline__ float block_max(const f32x16& s) {
     float top = fmaxf(s[0], s[1]);
 #pragma unroll
     for (int i = 2; i < 16; i += 2) top = fmaxf(top, fmaxf(s[i], s[i + 1]));
-    top = pair_max(top) * c;
+    return pair_max(top);
+}
+
+// Scores of a block -> P (16 bits), with the row's reference point, denominator and O kept up.
+template <bool F16, int MODE>
+__device__ __forceinline__ void softmax_block(const MaskArgs& a, f32x16& s, RowState& st, bf16x8 (&p)[2]) {
+    const float c = MODE == kPlain ? a.scale_log2 : 1.0f;
+    const float top = block_max(s) * c;
     const bool move = top > st.m + kTau; // (from -infinity: any score)
     if (__builtin_amdgcn_ballot_w64(move) != 0) {
         const float m = move ? top : st.m;
@@ -265,16 +279,16 @@ struct FragLane {
     unsigned v[4]; // of its V patch: dims 32 b .. + 31, key 4 h + (lane & 15) / 4 (and 8, 16, 24 further)
 };
 
-__device__ __forceinline__ bf16x8 k_frag(unsigned k_lds, const FragLane& fl, int t) { return *(lds_frag_t)(k_lds + fl.k[t]); }
+__device__ __forceinline__ bf16x8 k_frag(unsigned k_lds, const FragLane& fl, int t) { return *(lds_frag_t)(fl.k[t] + k_lds); }
 __device__ __forceinline__ s16x8 v_frag(unsigned v_lds, const FragLane& fl, int kb, int b) {
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t)(v_lds + fl.v[b] + (unsigned)(16 * kb * kRow)));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t)(v_lds + fl.v[b] + (unsigned)((16 * kb + 8) * kRow)));
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t)(fl.v[b] + v_lds + (unsigned)(16 * kb * kRow)));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t)(fl.v[b] + v_lds + (unsigned)((16 * kb + 8) * kRow)));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
 // One row by itself, all lanes of a wave: reference point, denominator and dims 2 lane, 2 lane + 1. Only the keys it sees
 // are read. Slow; for rows whose tile met numbers that are not finite.
-template <bool F16, bool FANCY>
+template <bool F16, int MODE>
 __device__ void row_alone(const MaskArgs& a, const KeySpan& sp, const SpanBase& base, const char* q, int lo, int hi, int pos, float slope, int lane, float& m,
                           float& l, float& o0, float& o1) {
     auto pair = [](const char* p, float& x, float& y) __attribute__((always_inline)) {
@@ -301,8 +315,7 @@ __device__ void row_alone(const MaskArgs& a, const KeySpan& sp, const SpanBase& 
         float s = q0 * k0 + q1 * k1;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o);
-        if constexpr (FANCY) s = fancy_score(a, s, slope, (float)(pos - j));
-        else s *= a.scale_log2;
+        s = MODE == kPlain ? s * a.scale_log2 : score_of<MODE>(a, s, slope, (float)(pos - j));
         if (!(s <= m)) { // (a NaN moves the reference to NaN, and stays)
             const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - s);
             m = s;
@@ -330,12 +343,96 @@ __device__ __forceinline__ unsigned round2(float x, float y) {
     }
 }
 
-template <bool F16, bool FANCY>
-__global__ void __launch_bounds__(256, 2) attn_masked_kernel(const MaskArgs a) {
+// The workgroup's place: sequence, key head, tile of rows, share of the keys.
+struct Item {
+    int sk, seq, kvh, tile, split;
+};
+__device__ __forceinline__ Item item_of(const MaskArgs& a, const MaskJob& job, int id) {
+    // consecutive items (tiles and shares of one head) on one XCD, whose L2 then holds the head's keys
+    const int xcd = id & 7, idx = id >> 3, per = job.workgroups >> 3, rem = job.workgroups & 7;
+    const int item = idx + xcd * per + min(xcd, rem);
+    Item it;
+    it.split = item % job.splits;
+    const int rest = item / job.splits;
+    it.tile = job.row_tiles - 1 - rest % job.row_tiles; // the last rows see the most keys: first
+    it.sk = rest / job.row_tiles;
+    it.kvh = it.sk % a.kv_heads;
+    it.seq = it.sk / a.kv_heads;
+    return it;
+}
+
+// Where a row's output, or its part, goes.
+struct RowOut {
+    const MaskArgs& a;
+    const MaskJob& job;
+    Item it;
+    int64_t part; // first row of the workgroup's parts
+    __device__ RowOut(const MaskArgs& args, const MaskJob& j, const Item& i, int tile_rows)
+        : a(args), job(j), it(i), part(j.part_base + ((int64_t)(i.sk * j.row_tiles + i.tile) * j.splits + i.split) * tile_rows) {}
+    __device__ __forceinline__ char* out(int row) const {
+        const RowPos p = row_pos(a, job, it.seq, row);
+        return a.o + (int64_t)p.seq * a.o_ss + (int64_t)p.tok * a.o_ts + (int64_t)(it.kvh * a.group + p.g) * a.o_hs;
+    }
+    __device__ __forceinline__ const char* q(int row) const {
+        const RowPos p = row_pos(a, job, it.seq, row);
+        return a.q + (int64_t)p.seq * a.q_ss + (int64_t)p.tok * a.q_ts + (int64_t)(it.kvh * a.group + p.g) * a.q_hs;
+    }
+    __device__ __forceinline__ float* part_o(int r) const { return a.part_o + (part + r) * D; }
+    __device__ __forceinline__ float* part_ml(int r) const { return a.part_ml + (part + r) * 2; }
+};
+
+// Rows row0 + bit of `bad` (part rows part0 + bit), each by itself over the keys [first, end) that its workgroup walks.
+template <bool F16, int MODE>
+__device__ __forceinline__ void rows_alone(const MaskArgs& a, const RowOut& to, unsigned bad, int row0, int part0, const int (&first)[2], const int (&end)[2],
+                                           float slope, int lane) {
+    bad = __builtin_amdgcn_readfirstlane(bad);
+#pragma clang loop unroll(disable)
+    while (bad != 0) {
+        const int x = __builtin_ctz(bad);
+        bad &= bad - 1;
+        const char* const q = to.q(row0 + x);
+        float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
+        const float sl = lane_f(slope, x);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            if (i >= to.job.spans) break;
+            const KeySpan& sp = to.job.span[i];
+            const Range r = row_range(a, to.job.kind[i], sp, row_pos(a, to.job, to.it.seq, row0 + x));
+            row_alone<F16, MODE>(a, sp, span_base(sp, to.it.seq, to.it.kvh), q, max(r.lo, first[i]), min(r.hi, end[i]), r.pos, sl, lane, m, l, o0, o1);
+        }
+        if (a.direct) {
+            const float inv = l == 0.f ? 0.f : 1.0f / l;
+            *reinterpret_cast<unsigned*>(to.out(row0 + x) + 4 * lane) = round2<F16>(o0 * inv, o1 * inv);
+        } else {
+            to.part_o(part0 + x)[2 * lane] = o0;
+            to.part_o(part0 + x)[2 * lane + 1] = o1;
+            if (lane == 0) {
+                to.part_ml(part0 + x)[0] = m;
+                to.part_ml(part0 + x)[1] = l;
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ void lane_offsets(int lane, FragLane& fl) {
+    const int l32 = lane & 31, h = lane >> 5, tr = (lane & 15) >> 2;
+#pragma unroll
+    for (int s = 0; s < 8; s++) fl.k[s] = (unsigned)(l32 * kRow + ((2 * s + h) ^ (l32 & 15)) * 16);
+#pragma unroll
+    for (int b = 0; b < 4; b++) fl.v[b] = (unsigned)((4 * h + tr) * kRow + ((b ^ tr) * 32 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2);
+}
+
+// 128 rows a workgroup, 32 a wave; every key block serves all four waves. Bound by the matrix unit and the softmax's
+// vector work, which run side by side: a step forms S(b + 1) = K(b + 1) Q^T and O += V(b - 1)^T P(b - 1) while the vector unit
+// turns S(b) into P(b). The three are independent, and 16 slots of one matrix instruction and one score each lay them out.
+// K and V have a ring of four blocks each; step b requests K(b + 4) and V(b + 2), both three steps ahead of their use, into
+// the stages that the step before has read for the last time, so one barrier a step orders all of it.
+// A reference point that moves in step b rescales O at its end: what P(b - 1) adds in it still goes by the old one.
+template <bool F16, int MODE>
+__global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, const int which) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     __shared__ int s_lo[2][4], s_hi[2][4];
-    __shared__ float s_ml[4][KB][2];
-    __shared__ unsigned s_bad;
+    constexpr unsigned kV = kStages * kBlock; // the V ring behind the K ring
 
     const int tid = threadIdx.x;
     const int lane = tid & 63;
@@ -343,49 +440,26 @@ __global__ void __launch_bounds__(256, 2) attn_masked_kernel(const MaskArgs a) {
     const int l32 = lane & 31;
     const int h = lane >> 5;
     const unsigned lds0 = __builtin_amdgcn_readfirstlane(lds_address(smem));
-
-    // ---- which rows, which keys
-    const int which = (int)blockIdx.x >= a.job[0].workgroups ? 1 : 0;
     const MaskJob& job = a.job[which];
-    int item;
-    {
-        // consecutive items (tiles and shares of one head) on one XCD, whose L2 then holds the head's keys
-        const int w = (int)blockIdx.x - (which ? a.job[0].workgroups : 0);
-        const int xcd = w & 7, idx = w >> 3, per = job.workgroups >> 3, rem = job.workgroups & 7;
-        item = idx + xcd * per + min(xcd, rem);
-    }
-    const int split = item % job.splits;
-    const int rest = item / job.splits;
-    const int tile = job.row_tiles - 1 - rest % job.row_tiles; // the last rows see the most keys: first
-    const int sk = rest / job.row_tiles;
-    const int kvh = sk % a.kv_heads;
-    const int seq = sk / a.kv_heads;
-    const bool by_keys = job.by_keys != 0;
-    const int tile_rows = by_keys ? kMaskRowsByKeys : kMaskRowsByWave;
-    const int row0 = tile * tile_rows + (by_keys ? 0 : 32 * wave);
+    const Item it = item_of(a, job, (int)blockIdx.x);
+    const RowOut to(a, job, it, kMaskRowsByWave);
+    const int row0 = it.tile * kMaskRowsByWave + 32 * wave;
     const int row = min(row0 + l32, job.rows - 1); // rows past the end work on the last one and are not written
-    const RowPos rp = row_pos(a, job, seq, row);
-    const int head = kvh * a.group + rp.g;
-    const float slope = (FANCY && a.slopes) ? a.slopes[head] * 1.4426950408889634f : 0.0f;
+    const RowPos rp = row_pos(a, job, it.seq, row);
+    const int head = it.kvh * a.group + rp.g;
+    const float slope = (MODE != kPlain && a.slopes) ? a.slopes[head] * 1.4426950408889634f : 0.0f;
+    const float c = MODE == kPlain ? a.scale_log2 : 1.0f;
 
     const char* const qrow = a.q + (int64_t)rp.seq * a.q_ss + (int64_t)rp.tok * a.q_ts + (int64_t)head * a.q_hs;
     bf16x8 qf[8];
 #pragma unroll
     for (int s = 0; s < 8; s++) qf[s] = *reinterpret_cast<const bf16x8*>(qrow + 32 * s + 16 * h);
-
     FragLane fl;
+    lane_offsets(lane, fl);
 #pragma unroll
-    for (int s = 0; s < 8; s++) fl.k[s] = (unsigned)(l32 * kRow + ((2 * s + h) ^ (l32 & 15)) * 16);
-    {
-        const int tr = (lane & 15) >> 2;
+    for (int s = 0; s < 8; s++) fl.k[s] += lds0;
 #pragma unroll
-        for (int b = 0; b < 4; b++) fl.v[b] = (unsigned)((4 * h + tr) * kRow + ((b ^ tr) * 32 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2);
-    }
-    LoadLane ln;
-    ln.q = (unsigned)lane >> 4;
-#pragma unroll
-    for (int n = 0; n < 4; n++) ln.kc[n] = (((unsigned)lane & 15u) ^ (4u * n + ln.q)) * 16u;
-    ln.vc = (((unsigned)lane & 15u) ^ (ln.q << 2)) * 16u;
+    for (int b = 0; b < 4; b++) fl.v[b] += lds0 + kV;
 
     RowState st;
     st.m = -INFINITY;
@@ -396,281 +470,422 @@ __global__ void __launch_bounds__(256, 2) attn_masked_kernel(const MaskArgs a) {
         for (int i = 0; i < 16; i++) st.o[b][i] = 0.f;
     bool live = true;
     int first[2] = {0, 0}, end[2] = {0, 0}; // the keys of each span that this workgroup walks
-    Range range[2];
 
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        range[i] = Range{0, 0, 0, true};
-        if (i >= job.spans) break;
+#pragma clang loop unroll(disable)
+    for (int i = 0; i < job.spans; i++) {
         const KeySpan& sp = job.span[i];
         const Range r = row_range(a, job.kind[i], sp, rp);
-        range[i] = r;
         live = r.live;
         const bool some = r.hi > r.lo;
         const int own_lo = wave_min(some ? r.lo : 0x7fffffff), own_hi = wave_max(some ? r.hi : 0);
         const int all_lo = wave_max(r.lo), all_hi = wave_min(r.hi); // what every row of the wave sees
-        int lo = own_lo, hi = own_hi;
-        if (!by_keys) {
-            if (lane == 0) {
-                s_lo[i][wave] = lo;
-                s_hi[i][wave] = hi;
-            }
-            __syncthreads();
-            lo = min(min(s_lo[i][0], s_lo[i][1]), min(s_lo[i][2], s_lo[i][3]));
-            hi = max(max(s_hi[i][0], s_hi[i][1]), max(s_hi[i][2], s_hi[i][3]));
-            lo = __builtin_amdgcn_readfirstlane(lo);
-            hi = __builtin_amdgcn_readfirstlane(hi);
+        if (lane == 0) {
+            s_lo[i][wave] = own_lo;
+            s_hi[i][wave] = own_hi;
         }
-        if (hi <= lo) continue; // no row sees a key of this span
-        int nb = (hi - lo + KB - 1) / KB;
+        __syncthreads();
+        int lo = min(min(s_lo[i][0], s_lo[i][1]), min(s_lo[i][2], s_lo[i][3]));
+        int hi = max(max(s_hi[i][0], s_hi[i][1]), max(s_hi[i][2], s_hi[i][3]));
+        lo = __builtin_amdgcn_readfirstlane(lo);
+        hi = __builtin_amdgcn_readfirstlane(hi);
+        int nb = hi > lo ? (hi - lo + KB - 1) / KB : 0;
         if (job.splits > 1) {
             const int per = (nb + job.splits - 1) / job.splits;
-            lo += split * per * KB;
-            nb = max(min(per, nb - split * per), 0);
+            lo += it.split * per * KB;
+            nb = max(min(per, nb - it.split * per), 0);
         }
         hi = min(hi, lo + nb * KB);
-        if (nb == 0) continue;
-        first[i] = lo;
-        end[i] = hi;
-        const int last = hi - 1;
-        const SpanBase base = span_base(sp, seq, kvh);
-        ln.k_ts = (unsigned)sp.k_ts;
-        ln.v_ts = (unsigned)sp.v_ts;
-
-        if (!by_keys) {
-            auto fetch = [&](int b) __attribute__((always_inline)) {
-                const unsigned at = lds0 + (unsigned)(b & (kStages - 1)) * (2u * kBlock);
-                load_rows<true, true>(sp, base, ln, lo + b * KB + 8 * wave, last, 2 * wave, at, at + kBlock);
-                load_rows<true, true>(sp, base, ln, lo + b * KB + 8 * wave + 4, last, 2 * wave + 1, at, at + kBlock);
-            };
-            fetch(0);
-            fetch(1);
-            fetch(2);
-#pragma clang loop unroll(disable)
-            for (int b = 0; b < nb; b++) {
-                asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" : : : "memory");
-                fetch(b + 3);
-                const int j0 = lo + b * KB;
-                if (j0 >= own_hi || j0 + KB <= own_lo) continue; // no row of this wave sees the block
-                const unsigned kl = lds0 + (unsigned)(b & (kStages - 1)) * (2u * kBlock), vl = kl + kBlock;
-                f32x16 s;
-#pragma unroll
-                for (int j = 0; j < 16; j++) s[j] = 0.f;
-#pragma unroll
-                for (int t = 0; t < 8; t++) s = mfma<F16>(k_frag(kl, fl, t), qf[t], s);
-                bf16x8 p[2];
-                softmax_block<F16, FANCY>(a, s, j0, h, r, slope, j0 >= all_lo && j0 + KB <= all_hi, st, p);
-#pragma unroll
-                for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-                    for (int d = 0; d < 4; d++) st.o[d] = mfma<F16>(__builtin_bit_cast(bf16x8, v_frag(vl, fl, kb, d)), p[kb], st.o[d]);
-            }
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
+        if (i == 0) {
+            first[0] = lo;
+            end[0] = hi;
         } else {
-            const unsigned kl = lds0 + (unsigned)wave * (2u * kBlock), vl = kl + kBlock;
-            if (wave < nb) {
-#pragma unroll
-                for (int n = 0; n < 8; n++) load_rows<true, false>(sp, base, ln, lo + wave * KB + 4 * n, last, n, kl, vl);
-#pragma unroll
-                for (int n = 0; n < 8; n++) load_rows<false, true>(sp, base, ln, lo + wave * KB + 4 * n, last, n, kl, vl);
-            }
-#pragma clang loop unroll(disable)
-            for (int b = wave; b < nb; b += 4) {
-                const bool more = b + 4 < nb;
-                const int j0 = lo + b * KB;
-                wait_loads<8>(); // K has arrived, V may be on its way
-                bf16x8 kf[8];
-#pragma unroll
-                for (int t = 0; t < 8; t++) kf[t] = k_frag(kl, fl, t);
-                asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-                if (more) {
-#pragma unroll
-                    for (int n = 0; n < 8; n++) load_rows<true, false>(sp, base, ln, j0 + 4 * KB + 4 * n, last, n, kl, vl);
-                }
-                f32x16 s;
-#pragma unroll
-                for (int j = 0; j < 16; j++) s[j] = 0.f;
-#pragma unroll
-                for (int t = 0; t < 8; t++) s = mfma<F16>(kf[t], qf[t], s);
-                bf16x8 p[2];
-                softmax_block<F16, FANCY>(a, s, j0, h, r, slope, j0 >= all_lo && j0 + KB <= all_hi, st, p);
-                if (more) wait_loads<8>();
-                else wait_loads<0>();
-                s16x8 vf[2][4];
-#pragma unroll
-                for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-                    for (int d = 0; d < 4; d++) vf[kb][d] = v_frag(vl, fl, kb, d);
-                asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-                if (more) {
-#pragma unroll
-                    for (int n = 0; n < 8; n++) load_rows<false, true>(sp, base, ln, j0 + 4 * KB + 4 * n, last, n, kl, vl);
-                }
-#pragma unroll
-                for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-                    for (int d = 0; d < 4; d++) st.o[d] = mfma<F16>(__builtin_bit_cast(bf16x8, vf[kb][d]), p[kb], st.o[d]);
-            }
+            first[1] = lo;
+            end[1] = hi;
         }
+        if (nb <= 0) continue; // no row sees a key of this span (or of this share of it)
+        const int last = hi - 1;
+        const SpanBase base = span_base(sp, it.seq, it.kvh);
+        // this wave's eight rows of a block: two loads each of K and V, four rows a load
+        const unsigned lq = (unsigned)lane >> 4;
+        const unsigned ko0 = lq * (unsigned)sp.k_ts + k_chunk(lane, 2 * wave), ko1 = (lq + 4) * (unsigned)sp.k_ts + k_chunk(lane, 2 * wave + 1);
+        const unsigned vo0 = lq * (unsigned)sp.v_ts + v_chunk(lane), vo1 = vo0 + 4 * (unsigned)sp.v_ts;
+        const int whole_blocks = base.table ? 0 : (hi - lo) / KB; // those that lie in memory as they do in LDS
+        const char* kp = base.k + (int64_t)(lo + 8 * wave) * sp.k_ts;
+        const char* vp = base.v + (int64_t)(lo + 8 * wave) * sp.v_ts;
+        const int64_t k_step = (int64_t)KB * sp.k_ts, v_step = (int64_t)KB * sp.v_ts;
+        const unsigned lds_w = lds0 + (unsigned)wave * 2048u;
+        auto fetch_k = [&](int b) __attribute__((always_inline)) {
+            const unsigned at = lds_w + (unsigned)(b & (kStages - 1)) * (unsigned)kBlock;
+            if (b < whole_blocks) {
+                rows_to_lds(kp, ko0, at);
+                rows_to_lds(kp, ko1, at + 1024u);
+                kp += k_step;
+            } else {
+                const int ln = lane_again();
+                load_rows<false>(sp, base, ln, lo + b * KB + 8 * wave, last, 2 * wave, at - (unsigned)wave * 2048u);
+                load_rows<false>(sp, base, ln, lo + b * KB + 8 * wave + 4, last, 2 * wave + 1, at - (unsigned)wave * 2048u);
+            }
+        };
+        auto fetch_v = [&](int b) __attribute__((always_inline)) {
+            const unsigned at = lds_w + kV + (unsigned)(b & (kStages - 1)) * (unsigned)kBlock;
+            if (b < whole_blocks) {
+                rows_to_lds(vp, vo0, at);
+                rows_to_lds(vp, vo1, at + 1024u);
+                vp += v_step;
+            } else {
+                const int ln = lane_again();
+                load_rows<true>(sp, base, ln, lo + b * KB + 8 * wave, last, 2 * wave, at - (unsigned)wave * 2048u);
+                load_rows<true>(sp, base, ln, lo + b * KB + 8 * wave + 4, last, 2 * wave + 1, at - (unsigned)wave * 2048u);
+            }
+        };
+        // P(-1) = 0 meets the V stage of "block -1", which has to hold finite numbers
+        for (int z = tid; z < kBlock / 16; z += 256) *reinterpret_cast<u32x4*>(smem + kV + (kStages - 1) * kBlock + 16 * z) = u32x4{0u, 0u, 0u, 0u};
+        fetch_k(0);
+        fetch_k(1);
+        fetch_k(2);
+        fetch_v(0);
+        fetch_k(3);
+        fetch_v(1);
+        asm volatile("s_waitcnt vmcnt(10) lgkmcnt(0)\n\ts_barrier" : : : "memory");
+        f32x16 s_a, s_b;
+        bf16x8 p_a[2], p_b[2];
+        const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        s_a = zero;
+#pragma unroll
+        for (int t = 0; t < 8; t++) s_a = mfma<F16>(k_frag(0, fl, t), qf[t], s_a);
+        p_a[0] = p_a[1] = __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u});
+        auto finish_scores = [&](f32x16& s, int b) __attribute__((always_inline)) {
+            const int j0 = lo + b * KB;
+            score_block<MODE>(a, s, j0, h, r.pos, slope);
+            if (!(j0 >= all_lo && j0 + KB <= all_hi)) mask_block(s, j0, h, r);
+        };
+        // The reference point at a block's maximum, where that is higher: what was summed goes by the new one.
+        auto raise = [&](const f32x16& s) __attribute__((always_inline)) {
+            const float m = fmaxf(st.m, block_max(s) * c);
+            const float f = st.m == m ? 1.0f : __builtin_amdgcn_exp2f(st.m - m);
+            st.m = m;
+            st.l *= f;
+#pragma unroll
+            for (int d = 0; d < 4; d++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) st.o[d][j] *= f;
+        };
+        finish_scores(s_a, 0);
+        raise(s_a);
+
+        auto step = [&](auto phase, int b, f32x16& s, f32x16& s_next, const bf16x8 (&p_old)[2], bf16x8 (&p)[2]) __attribute__((always_inline)) {
+            constexpr int J = decltype(phase)::value;
+            const unsigned k_at = (unsigned)(((J >= 0 ? J : b) + 1) & 3) * (unsigned)kBlock, v_at = (unsigned)(((J >= 0 ? J : b) + 3) & 3) * (unsigned)kBlock;
+            // (address + stage is an immediate of the read only where it is formed here, not ahead of the loop for every stage)
+#pragma unroll
+            for (int x = 0; x < 8; x++) pin(fl.k[x]);
+#pragma unroll
+            for (int x = 0; x < 4; x++) pin(fl.v[x]);
+            asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" : : : "memory");
+            fetch_k(b + 4);
+            fetch_v(b + 2);
+            bf16x8 kf[8];
+            s16x8 vf[8];
+            constexpr int LA = 3; // slots between a fragment's read and its use
+            auto read = [&](int slot) __attribute__((always_inline)) {
+                if (slot & 1) vf[slot >> 1] = v_frag(v_at, fl, slot >> 3, (slot >> 1) & 3);
+                else kf[slot >> 1] = k_frag(k_at, fl, slot >> 1);
+            };
+#pragma unroll
+            for (int x = 0; x < LA; x++) read(x);
+            const float ref = st.m == -INFINITY ? 0.0f : st.m;
+            float sum = 0.f, e[16];
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int x = 0; x < 16; x++) {
+                if (x + LA < 16) read(x + LA);
+                if (x & 1) st.o[(x >> 1) & 3] = mfma<F16>(__builtin_bit_cast(bf16x8, vf[x >> 1]), p_old[x >> 3], st.o[(x >> 1) & 3]);
+                else s_next = mfma<F16>(kf[x >> 1], qf[x >> 1], x == 0 ? zero : s_next);
+                e[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x], c, -ref));
+                sum += e[x];
+                pin(sum);
+                if ((x & 7) == 7) {
+                    p[x >> 3] = round8<F16>(e, x - 7);
+                    pin(p[x >> 3]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            // a score far above the reference point, a number that is none, or the first block that a row sees
+            const int j0 = lo + b * KB;
+            if (__builtin_amdgcn_ballot_w64(!(sum <= kLimit) || (st.m == -INFINITY && r.lo < j0 + KB && r.hi > j0)) != 0) {
+                raise(s);
+                const float ref2 = st.m == -INFINITY ? 0.0f : st.m;
+                sum = 0.f;
+#pragma unroll
+                for (int x = 0; x < 16; x++) {
+                    e[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x], c, -ref2));
+                    sum += e[x];
+                }
+                p[0] = round8<F16>(e, 0);
+                p[1] = round8<F16>(e, 8);
+            }
+            st.l += sum;
+            finish_scores(s_next, b + 1);
+        };
+        int b = 0;
+#pragma clang loop unroll(disable)
+        for (; b + 4 <= nb; b += 4) {
+            step(std::integral_constant<int, 0>{}, b, s_a, s_b, p_a, p_b);
+            step(std::integral_constant<int, 1>{}, b + 1, s_b, s_a, p_b, p_a);
+            step(std::integral_constant<int, 2>{}, b + 2, s_a, s_b, p_a, p_b);
+            step(std::integral_constant<int, 3>{}, b + 3, s_b, s_a, p_b, p_a);
+        }
+#pragma clang loop unroll(disable)
+        for (; b < nb; b++) {
+            step(std::integral_constant<int, -1>{}, b, s_a, s_b, p_a, p_b);
+            s_a = s_b;
+            p_a[0] = p_b[0];
+            p_a[1] = p_b[1];
+        }
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
+        {
+            const unsigned v_at = (unsigned)((nb - 1) & (kStages - 1)) * (unsigned)kBlock;
+#pragma unroll
+            for (int x = 0; x < 8; x++) st.o[x & 3] = mfma<F16>(__builtin_bit_cast(bf16x8, v_frag(v_at, fl, x >> 2, x & 3)), p_a[x >> 2], st.o[x & 3]);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory"); // the rings are free again
     }
     st.l = pair_sum(st.l);
 
     // ---- the rows leave: through LDS, so that they are stored as whole rows
     const bool here = live && row0 + l32 < job.rows;
-    float* const part_o = a.part_o + (job.part_base + ((int64_t)(sk * job.row_tiles + tile) * job.splits + split) * tile_rows) * D;
-    float* const part_ml = a.part_ml + (job.part_base + ((int64_t)(sk * job.row_tiles + tile) * job.splits + split) * tile_rows) * 2;
-    unsigned bad = 0; // rows of this wave's 32 (by_keys: of the workgroup's) to be formed again
-
-    if (!by_keys) {
-        float z = 0.f;
+    float z = 0.f;
+#pragma unroll
+    for (int b = 0; b < 4; b++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) z = __builtin_fmaf(st.o[b][i], 0.0f, z);
+    z = pair_sum(__builtin_fmaf(st.l, 0.0f, z));
+    const unsigned bad = (unsigned)__builtin_amdgcn_ballot_w64(here && !(z == 0.0f));
+    if (a.direct) {
+        const float inv = st.l > 0.f ? 1.0f / st.l : 0.f;
+        unsigned char* const mine = smem + wave * (32 * kRow); // (the rings are idle; 16-byte chunks swizzled by row)
 #pragma unroll
         for (int b = 0; b < 4; b++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) z = __builtin_fmaf(st.o[b][i], 0.0f, z);
-        z = __builtin_fmaf(st.l, 0.0f, z);
-        z = pair_sum(z);
-        bad = (unsigned)__builtin_amdgcn_ballot_w64(here && !(z == 0.0f));
-        if (a.direct) {
-            const float inv = st.l > 0.f ? 1.0f / st.l : 0.f;
-            unsigned char* const mine = smem + wave * (32 * kRow); // (the ring is idle; 16-byte chunks swizzled by row)
+            for (int i = 0; i < 4; i++) {
+                const u32x2 w = {round2<F16>(st.o[b][4 * i] * inv, st.o[b][4 * i + 1] * inv), round2<F16>(st.o[b][4 * i + 2] * inv, st.o[b][4 * i + 3] * inv)};
+                *reinterpret_cast<u32x2*>(mine + l32 * kRow + (((4 * b + i) ^ (l32 & 15)) * 16) + 8 * h) = w;
+            }
+        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+        const unsigned good = (unsigned)__builtin_amdgcn_ballot_w64(here) & ~bad;
+#pragma unroll
+        for (int n = 0; n < 8; n++) {
+            const int rr = 4 * n + (lane >> 4);
+            const u32x4 w = *reinterpret_cast<const u32x4*>(mine + rr * kRow + (((lane & 15) ^ (rr & 15)) * 16));
+            if ((good >> rr) & 1u) *reinterpret_cast<u32x4*>(to.out(row0 + rr) + 16 * (lane & 15)) = w;
+        }
+    } else if (here) {
+        const int at = 32 * wave + l32;
+        if (st.l != 0.f) {
 #pragma unroll
             for (int b = 0; b < 4; b++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const u32x2 w = {round2<F16>(st.o[b][4 * i] * inv, st.o[b][4 * i + 1] * inv), round2<F16>(st.o[b][4 * i + 2] * inv, st.o[b][4 * i + 3] * inv)};
-                    *reinterpret_cast<u32x2*>(mine + l32 * kRow + (((4 * b + i) ^ (l32 & 15)) * 16) + 8 * h) = w;
-                }
-            asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-            const unsigned good = (unsigned)__builtin_amdgcn_ballot_w64(here) & ~bad;
-#pragma unroll
-            for (int n = 0; n < 8; n++) {
-                const int rr = 4 * n + (lane >> 4);
-                const u32x4 w = *reinterpret_cast<const u32x4*>(mine + rr * kRow + (((lane & 15) ^ (rr & 15)) * 16));
-                if ((good >> rr) & 1u) {
-                    const RowPos p = row_pos(a, job, seq, row0 + rr);
-                    char* const out = a.o + (int64_t)p.seq * a.o_ss + (int64_t)p.tok * a.o_ts + (int64_t)(kvh * a.group + p.g) * a.o_hs;
-                    *reinterpret_cast<u32x4*>(out + 16 * (lane & 15)) = w;
-                }
-            }
-        } else {
-            const int at = 32 * wave + l32;
-            if (here && st.l != 0.f) {
-#pragma unroll
-                for (int b = 0; b < 4; b++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        *reinterpret_cast<f32x4*>(part_o + (int64_t)at * D + 32 * b + 8 * i + 4 * h) =
-                            f32x4{st.o[b][4 * i], st.o[b][4 * i + 1], st.o[b][4 * i + 2], st.o[b][4 * i + 3]};
-            }
-            if (here && h == 0) {
-                part_ml[2 * at] = st.m;
-                part_ml[2 * at + 1] = st.l;
-            }
+                for (int i = 0; i < 4; i++)
+                    *reinterpret_cast<f32x4*>(to.part_o(at) + 32 * b + 8 * i + 4 * h) = f32x4{st.o[b][4 * i], st.o[b][4 * i + 1], st.o[b][4 * i + 2], st.o[b][4 * i + 3]};
         }
-    } else {
-        // the four waves' shares of the same rows, joined in their order
-        if (tid == 0) s_bad = 0;
         if (h == 0) {
-            s_ml[wave][l32][0] = st.m;
-            s_ml[wave][l32][1] = st.l;
+            to.part_ml(at)[0] = st.m;
+            to.part_ml(at)[1] = st.l;
         }
-        unsigned char* const mine = smem + wave * (2 * kBlock); // 32 x 512 bytes, 16-byte chunks swizzled by row
+    }
+    if (bad != 0) {
+        asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); // what is formed again comes behind what was stored
+        rows_alone<F16, MODE>(a, to, bad, row0, 32 * wave, first, end, slope, lane);
+    }
+}
+
+// 32 rows a workgroup; its four waves take the key blocks in turn, each through 16 KB of its own without a barrier, and
+// are joined at the end. Bound by the keys' bytes where rows are few: K of the next block is requested as soon as this
+// one's fragments are in registers, V likewise, so that 8 to 16 KB a wave, eight waves a CU, are always on their way.
+template <bool F16, int MODE>
+__global__ void __launch_bounds__(256, 2) attn_keys_kernel(const MaskArgs a, const int which0) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    __shared__ float s_ml[4][KB][2];
+    __shared__ unsigned s_bad;
+
+    const int tid = threadIdx.x;
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l32 = lane & 31;
+    const int h = lane >> 5;
+    const unsigned lds0 = __builtin_amdgcn_readfirstlane(lds_address(smem));
+    // (two jobs of this form are one launch)
+    const bool second = (int)blockIdx.x >= a.job[which0].workgroups;
+    const MaskJob& job = a.job[second ? 1 : which0];
+    const Item it = item_of(a, job, (int)blockIdx.x - (second ? a.job[0].workgroups : 0));
+    const RowOut to(a, job, it, kMaskRowsByKeys);
+    const int row0 = it.tile * kMaskRowsByKeys;
+    const int row = min(row0 + l32, job.rows - 1);
+    const RowPos rp = row_pos(a, job, it.seq, row);
+    const int head = it.kvh * a.group + rp.g;
+    const float slope = (MODE != kPlain && a.slopes) ? a.slopes[head] * 1.4426950408889634f : 0.0f;
+
+    const char* const qrow = a.q + (int64_t)rp.seq * a.q_ss + (int64_t)rp.tok * a.q_ts + (int64_t)head * a.q_hs;
+    bf16x8 qf[8];
 #pragma unroll
-        for (int b = 0; b < 4; b++)
+    for (int s = 0; s < 8; s++) qf[s] = *reinterpret_cast<const bf16x8*>(qrow + 32 * s + 16 * h);
+    FragLane fl;
+    lane_offsets(lane, fl);
+
+    RowState st;
+    st.m = -INFINITY;
+    st.l = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                *reinterpret_cast<f32x4*>(mine + l32 * (2 * kRow) + (((8 * b + 2 * i + h) ^ l32) * 16)) =
-                    f32x4{st.o[b][4 * i], st.o[b][4 * i + 1], st.o[b][4 * i + 2], st.o[b][4 * i + 3]};
-        __syncthreads();
-        const int rr = tid >> 3, c8 = tid & 7; // eight threads a row, 16 dims each
-        float m = -INFINITY;
+    for (int b = 0; b < 4; b++)
 #pragma unroll
-        for (int w = 0; w < 4; w++) m = fmaxf(m, s_ml[w][rr][0]);
-        float l = 0.f;
-        f32x4 o[4];
+        for (int i = 0; i < 16; i++) st.o[b][i] = 0.f;
+    bool live = true;
+    int first[2] = {0, 0}, end[2] = {0, 0};
+
+#pragma clang loop unroll(disable)
+    for (int i = 0; i < job.spans; i++) {
+        const KeySpan& sp = job.span[i];
+        const Range r = row_range(a, job.kind[i], sp, rp);
+        live = r.live;
+        const bool some = r.hi > r.lo;
+        int lo = wave_min(some ? r.lo : 0x7fffffff), hi = wave_max(some ? r.hi : 0);
+        const int all_lo = wave_max(r.lo), all_hi = wave_min(r.hi); // what every row sees
+        int nb = hi > lo ? (hi - lo + KB - 1) / KB : 0;
+        if (job.splits > 1) {
+            const int per = (nb + job.splits - 1) / job.splits;
+            lo += it.split * per * KB;
+            nb = max(min(per, nb - it.split * per), 0);
+        }
+        hi = min(hi, lo + nb * KB);
+        if (i == 0) {
+            first[0] = lo;
+            end[0] = hi;
+        } else {
+            first[1] = lo;
+            end[1] = hi;
+        }
+        if (nb <= 0) continue;
+        const int last = hi - 1;
+        const SpanBase base = span_base(sp, it.seq, it.kvh);
+        const unsigned kl = lds0 + (unsigned)wave * (2u * kBlock), vl = kl + kBlock;
+        if (wave < nb) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int n = 0; n < 8; n++) load_rows<false>(sp, base, lane, lo + wave * KB + 4 * n, last, n, kl);
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
-            const float mw = s_ml[w][rr][0], lw = s_ml[w][rr][1];
-            if (lw == 0.f) continue; // (a share without keys)
-            const float f = __builtin_amdgcn_exp2f(mw - m);
-            l += f * lw;
+            for (int n = 0; n < 8; n++) load_rows<true>(sp, base, lane, lo + wave * KB + 4 * n, last, n, vl);
+        }
+#pragma clang loop unroll(disable)
+        for (int b = wave; b < nb; b += 4) {
+            const bool more = b + 4 < nb;
+            const int j0 = lo + b * KB;
+            wait_loads<8>(); // K has arrived, V may be on its way
+            bf16x8 kf[8];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const f32x4 x = *reinterpret_cast<const f32x4*>(smem + w * (2 * kBlock) + rr * (2 * kRow) + (((4 * c8 + i) ^ rr) * 16));
+            for (int t = 0; t < 8; t++) kf[t] = k_frag(kl, fl, t);
+            asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+            if (more) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) o[i][j] = __builtin_fmaf(f, x[j], o[i][j]);
+                for (int n = 0; n < 8; n++) load_rows<false>(sp, base, lane, j0 + 4 * KB + 4 * n, last, n, kl);
             }
+            f32x16 s;
+#pragma unroll
+            for (int j = 0; j < 16; j++) s[j] = 0.f;
+#pragma unroll
+            for (int t = 0; t < 8; t++) s = mfma<F16>(kf[t], qf[t], s);
+            score_block<MODE>(a, s, j0, h, r.pos, slope);
+            if (!(j0 >= all_lo && j0 + KB <= all_hi)) mask_block(s, j0, h, r);
+            bf16x8 p[2];
+            softmax_block<F16, MODE>(a, s, st, p);
+            if (more) wait_loads<8>();
+            else wait_loads<0>();
+            s16x8 vf[2][4];
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                for (int d = 0; d < 4; d++) vf[kb][d] = v_frag(vl, fl, kb, d);
+            asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+            if (more) {
+#pragma unroll
+                for (int n = 0; n < 8; n++) load_rows<true>(sp, base, lane, j0 + 4 * KB + 4 * n, last, n, vl);
+            }
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                for (int d = 0; d < 4; d++) st.o[d] = mfma<F16>(__builtin_bit_cast(bf16x8, vf[kb][d]), p[kb], st.o[d]);
         }
-        float z = l * 0.0f;
+    }
+    st.l = pair_sum(st.l);
+
+    const bool here = live && row0 + l32 < job.rows;
+    // the four waves' shares of the same rows, joined in their order
+    if (tid == 0) s_bad = 0;
+    if (h == 0) {
+        s_ml[wave][l32][0] = st.m;
+        s_ml[wave][l32][1] = st.l;
+    }
+    unsigned char* const mine = smem + wave * (2 * kBlock); // 32 x 512 bytes, 16-byte chunks swizzled by row
+#pragma unroll
+    for (int b = 0; b < 4; b++)
 #pragma unroll
         for (int i = 0; i < 4; i++)
+            *reinterpret_cast<f32x4*>(mine + l32 * (2 * kRow) + (((8 * b + 2 * i + h) ^ l32) * 16)) =
+                f32x4{st.o[b][4 * i], st.o[b][4 * i + 1], st.o[b][4 * i + 2], st.o[b][4 * i + 3]};
+    __syncthreads();
+    const int rr = tid >> 3, c8 = tid & 7; // eight threads a row, 16 dims each
+    float m = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < 4; j++) z = __builtin_fmaf(o[i][j], 0.0f, z);
+    for (int w = 0; w < 4; w++) m = fmaxf(m, s_ml[w][rr][0]);
+    float l = 0.f;
+    f32x4 o[4];
 #pragma unroll
-        for (int x = 1; x < 8; x <<= 1) z += __shfl_xor(z, x);
-        const unsigned alive = (unsigned)__builtin_amdgcn_ballot_w64(here);
-        const bool mine_live = (alive >> rr) & 1u;
-        const bool again = mine_live && !(z == 0.f);
-        if (again && c8 == 0) atomicOr(&s_bad, 1u << rr);
-        if (mine_live && !again) {
-            if (a.direct) {
-                const float inv = l > 0.f ? 1.0f / l : 0.f;
-                const RowPos p = row_pos(a, job, seq, row0 + rr);
-                char* const out = a.o + (int64_t)p.seq * a.o_ss + (int64_t)p.tok * a.o_ts + (int64_t)(kvh * a.group + p.g) * a.o_hs + 32 * c8;
-                u32x4 w[2];
+    for (int i = 0; i < 4; i++) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    w[i >> 1][2 * (i & 1)] = round2<F16>(o[i][0] * inv, o[i][1] * inv);
-                    w[i >> 1][2 * (i & 1) + 1] = round2<F16>(o[i][2] * inv, o[i][3] * inv);
-                }
-                *reinterpret_cast<u32x4*>(out) = w[0];
-                *reinterpret_cast<u32x4*>(out + 16) = w[1];
-            } else {
+    for (int w = 0; w < 4; w++) {
+        const float mw = s_ml[w][rr][0], lw = s_ml[w][rr][1];
+        if (lw == 0.f) continue; // (a share without keys)
+        const float f = __builtin_amdgcn_exp2f(mw - m);
+        l += f * lw;
 #pragma unroll
-                for (int i = 0; i < 4; i++) *reinterpret_cast<f32x4*>(part_o + (int64_t)rr * D + 16 * c8 + 4 * i) = o[i];
-                if (c8 == 0) {
-                    part_ml[2 * rr] = m;
-                    part_ml[2 * rr + 1] = l;
-                }
-            }
+        for (int i = 0; i < 4; i++) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(smem + w * (2 * kBlock) + rr * (2 * kRow) + (((4 * c8 + i) ^ rr) * 16));
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[i][j] = __builtin_fmaf(f, x[j], o[i][j]);
         }
-        __syncthreads();
-        bad = s_bad;
-        bad &= 0x11111111u << wave; // every wave forms a quarter of them
     }
-
-    // ---- rows that met a number that is not finite
-    bad = __builtin_amdgcn_readfirstlane(bad);
-#pragma clang loop unroll(disable)
-    while (bad != 0) {
-        const int x = __builtin_ctz(bad);
-        bad &= bad - 1;
-        const RowPos p = row_pos(a, job, seq, row0 + x);
-        const char* const q = a.q + (int64_t)p.seq * a.q_ss + (int64_t)p.tok * a.q_ts + (int64_t)(kvh * a.group + p.g) * a.q_hs;
-        float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-        const float sl = lane_f(slope, x);
+    float z = l * 0.0f;
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            if (i >= job.spans) break;
-            const int lo = max(__builtin_amdgcn_readlane(range[i].lo, x), first[i]), hi = min(__builtin_amdgcn_readlane(range[i].hi, x), end[i]);
-            row_alone<F16, FANCY>(a, job.span[i], span_base(job.span[i], seq, kvh), q, lo, hi, __builtin_amdgcn_readlane(range[i].pos, x), sl, lane, m, l, o0, o1);
-        }
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) z = __builtin_fmaf(o[i][j], 0.0f, z);
+#pragma unroll
+    for (int x = 1; x < 8; x <<= 1) z += __shfl_xor(z, x);
+    const unsigned alive = (unsigned)__builtin_amdgcn_ballot_w64(here);
+    const bool mine_live = (alive >> rr) & 1u;
+    const bool again = mine_live && !(z == 0.f);
+    if (again && c8 == 0) atomicOr(&s_bad, 1u << rr);
+    if (mine_live && !again) {
         if (a.direct) {
-            const float inv = l == 0.f ? 0.f : 1.0f / l;
-            char* const out = a.o + (int64_t)p.seq * a.o_ss + (int64_t)p.tok * a.o_ts + (int64_t)(kvh * a.group + p.g) * a.o_hs;
-            *reinterpret_cast<unsigned*>(out + 4 * lane) = round2<F16>(o0 * inv, o1 * inv);
+            const float inv = l > 0.f ? 1.0f / l : 0.f;
+            char* const out = to.out(row0 + rr) + 32 * c8;
+            u32x4 w[2];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                w[i >> 1][2 * (i & 1)] = round2<F16>(o[i][0] * inv, o[i][1] * inv);
+                w[i >> 1][2 * (i & 1) + 1] = round2<F16>(o[i][2] * inv, o[i][3] * inv);
+            }
+            *reinterpret_cast<u32x4*>(out) = w[0];
+            *reinterpret_cast<u32x4*>(out + 16) = w[1];
         } else {
-            const int at = (by_keys ? 0 : 32 * wave) + x;
-            part_o[(int64_t)at * D + 2 * lane] = o0;
-            part_o[(int64_t)at * D + 2 * lane + 1] = o1;
-            if (lane == 0) {
-                part_ml[2 * at] = m;
-                part_ml[2 * at + 1] = l;
+#pragma unroll
+            for (int i = 0; i < 4; i++) *reinterpret_cast<f32x4*>(to.part_o(rr) + 16 * c8 + 4 * i) = o[i];
+            if (c8 == 0) {
+                to.part_ml(rr)[0] = m;
+                to.part_ml(rr)[1] = l;
             }
         }
     }
+    __syncthreads();
+    rows_alone<F16, MODE>(a, to, s_bad & (0x11111111u << wave), row0, 0, first, end, slope, lane); // (every wave a quarter of them)
 }
 
 // The shares of each row's keys, joined in their order: half a wave a row.
@@ -715,36 +930,56 @@ __global__ void __launch_bounds__(256) attn_masked_merge_kernel(const MaskArgs a
 
 } // namespace msk
 
-hipError_t masked_setup() {
-    const void* const fns[4] = {reinterpret_cast<const void*>(&msk::attn_masked_kernel<false, false>), reinterpret_cast<const void*>(&msk::attn_masked_kernel<false, true>),
-                                reinterpret_cast<const void*>(&msk::attn_masked_kernel<true, false>), reinterpret_cast<const void*>(&msk::attn_masked_kernel<true, true>)};
-    for (const void* f : fns) {
-        hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, msk::kLds);
+namespace {
+template <bool F16, int MODE>
+hipError_t launch_jobs(const MaskArgs& a, hipStream_t stream) {
+    const dim3 block(256);
+    if (a.jobs == 2 && a.job[0].by_keys && a.job[1].by_keys) {
+        msk::attn_keys_kernel<F16, MODE><<<dim3((unsigned)(a.job[0].workgroups + a.job[1].workgroups)), block, msk::kLds, stream>>>(a, 0);
+        return hipGetLastError();
+    }
+    for (int i = 0; i < a.jobs; i++) {
+        const dim3 grid((unsigned)a.job[i].workgroups);
+        if (a.job[i].by_keys) msk::attn_keys_kernel<F16, MODE><<<grid, block, msk::kLds, stream>>>(a, i);
+        else msk::attn_rows_kernel<F16, MODE><<<grid, block, msk::kLds, stream>>>(a, i);
+        const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
     return hipSuccess;
 }
 
-hipError_t launch_masked(const MaskArgs& a, hipStream_t stream) {
-    int wgs = 0;
-    for (int i = 0; i < a.jobs; i++) wgs += a.job[i].workgroups;
-    const bool fancy = a.cap_in != 0.0f || a.slopes != nullptr;
-    const dim3 grid((unsigned)wgs), block(256);
-    if (a.f16) {
-        if (fancy) msk::attn_masked_kernel<true, true><<<grid, block, msk::kLds, stream>>>(a);
-        else msk::attn_masked_kernel<true, false><<<grid, block, msk::kLds, stream>>>(a);
-    } else {
-        if (fancy) msk::attn_masked_kernel<false, true><<<grid, block, msk::kLds, stream>>>(a);
-        else msk::attn_masked_kernel<false, false><<<grid, block, msk::kLds, stream>>>(a);
-    }
-    hipError_t e = hipGetLastError();
+template <bool F16>
+hipError_t launch_typed(const MaskArgs& a, hipStream_t stream) {
+    const hipError_t e = a.cap_in != 0.0f ? launch_jobs<F16, msk::kCap>(a, stream) : a.slopes ? launch_jobs<F16, msk::kBias>(a, stream) : launch_jobs<F16, msk::kPlain>(a, stream);
     if (e != hipSuccess || a.direct) return e;
     const MaskJob& last = a.job[a.jobs - 1]; // tiled by sequence
     const int rows = last.seqs * a.kv_heads * last.rows;
-    const dim3 mgrid((unsigned)((rows + 7) / 8));
-    if (a.f16) msk::attn_masked_merge_kernel<true><<<mgrid, block, 0, stream>>>(a, rows);
-    else msk::attn_masked_merge_kernel<false><<<mgrid, block, 0, stream>>>(a, rows);
+    msk::attn_masked_merge_kernel<F16><<<dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, stream>>>(a, rows);
     return hipGetLastError();
 }
+
+template <bool F16, int MODE>
+hipError_t setup_one() {
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&msk::attn_rows_kernel<F16, MODE>), hipFuncAttributeMaxDynamicSharedMemorySize, msk::kLds);
+    if (e == hipSuccess) e = hipFuncSetAttribute(reinterpret_cast<const void*>(&msk::attn_keys_kernel<F16, MODE>), hipFuncAttributeMaxDynamicSharedMemorySize, msk::kLds);
+    return e;
+}
+} // namespace
+
+hipError_t masked_setup() {
+    hipError_t e = setup_one<false, msk::kPlain>();
+    if (e == hipSuccess) e = setup_one<false, msk::kBias>();
+    if (e == hipSuccess) e = setup_one<false, msk::kCap>();
+    if (e == hipSuccess) e = setup_one<true, msk::kPlain>();
+    if (e == hipSuccess) e = setup_one<true, msk::kBias>();
+    if (e == hipSuccess) e = setup_one<true, msk::kCap>();
+    return e;
+}
+
+int masked_launches(const MaskArgs& a) {
+    return (a.jobs == 2 && !(a.job[0].by_keys && a.job[1].by_keys) ? 2 : 1) + (a.direct ? 0 : 1);
+}
+
+hipError_t launch_masked(const MaskArgs& a, hipStream_t stream) { return a.f16 ? launch_typed<true>(a, stream) : launch_typed<false>(a, stream); }
 
 } // namespace zdraw

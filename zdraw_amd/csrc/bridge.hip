@@ -2107,7 +2107,7 @@ int enqueue_masked(Queue* qu, MaskArgs* a, size_t part_rows, void* workspace) {
         set_err("masked attention launch: %s", hipGetErrorString(e));
         return ZDRAW_HIP_ERR_HANDLE;
     }
-    g_dispatch += a->direct ? 1 : 2;
+    g_dispatch += masked_launches(*a);
     return ZDRAW_HIP_OK;
 }
 

@@ -67,6 +67,7 @@ constexpr int kMaskRowsByKeys = 32;
 
 hipError_t masked_setup();
 hipError_t launch_masked(const MaskArgs& a, hipStream_t stream);
+int masked_launches(const MaskArgs& a); // kernels of a call
 
 struct AppendArgs {
     const char* q; // null: no query rows
