@@ -128,6 +128,35 @@ __device__ __forceinline__ Range row_range(const MaskArgs& a, int kind, const Ke
     return r;
 }
 
+// What the rows of a wave see together: from the first to the last key of any row, and what every row sees. `first_row`,
+// `last_row`: of the wave's rows, held to the sequence. Without documents the ranges of a sequence's rows only grow.
+struct WaveRange {
+    int lo, hi, all_lo, all_hi;
+};
+__device__ __forceinline__ int wave_min(int x);
+__device__ __forceinline__ int wave_max(int x);
+__device__ __forceinline__ WaveRange wave_range(const MaskArgs& a, const MaskJob& job, int kind, const KeySpan& sp, int seq, int first_row, int last_row, const Range& r) {
+    WaveRange w;
+    if ((kind == kRangeDocs && a.q_starts) || (job.pooled && a.q_lens)) {
+        const bool some = r.hi > r.lo;
+        w.lo = wave_min(some ? r.lo : 0x7fffffff);
+        w.hi = wave_max(some ? r.hi : 0);
+        w.all_lo = wave_max(r.lo);
+        w.all_hi = wave_min(r.hi);
+        return w;
+    }
+    w.lo = w.all_lo = 0;
+    if (kind == kRangePrefix) {
+        // (rows past their request's are among those that "see" the prefix: they are not written)
+        w.hi = w.all_hi = sp.keys;
+        return w;
+    }
+    const Range lo = row_range(a, kind, sp, RowPos{seq, first_row / a.group, 0}), hi = row_range(a, kind, sp, RowPos{seq, last_row / a.group, 0});
+    w.all_hi = hi.live ? lo.hi : 0;
+    w.hi = hi.live ? hi.hi : wave_max(r.hi);
+    return w;
+}
+
 __device__ __forceinline__ int wave_min(int x) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) x = min(x, __shfl_xor(x, o));
@@ -348,14 +377,14 @@ struct Item {
     int sk, seq, kvh, tile, split;
 };
 __device__ __forceinline__ Item item_of(const MaskArgs& a, const MaskJob& job, int id) {
-    // consecutive items (tiles and shares of one head) on one XCD, whose L2 then holds the head's keys
+    // consecutive items on one XCD, whose L2 then serves the tiles that walk the same keys
     const int xcd = id & 7, idx = id >> 3, per = job.workgroups >> 3, rem = job.workgroups & 7;
     const int item = idx + xcd * per + min(xcd, rem);
     Item it;
-    it.split = item % job.splits;
-    const int rest = item / job.splits;
-    it.tile = job.row_tiles - 1 - rest % job.row_tiles; // the last rows see the most keys: first
-    it.sk = rest / job.row_tiles;
+    it.tile = job.row_tiles - 1 - item % job.row_tiles; // the last rows see the most keys: first
+    const int rest = item / job.row_tiles;
+    it.split = rest % job.splits;
+    it.sk = rest / job.splits;
     it.kvh = it.sk % a.kv_heads;
     it.seq = it.sk / a.kv_heads;
     return it;
@@ -476,12 +505,11 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
         const KeySpan& sp = job.span[i];
         const Range r = row_range(a, job.kind[i], sp, rp);
         live = r.live;
-        const bool some = r.hi > r.lo;
-        const int own_lo = wave_min(some ? r.lo : 0x7fffffff), own_hi = wave_max(some ? r.hi : 0);
-        const int all_lo = wave_max(r.lo), all_hi = wave_min(r.hi); // what every row of the wave sees
+        const WaveRange wr = wave_range(a, job, job.kind[i], sp, it.seq, min(row0, job.rows - 1), min(row0 + 31, job.rows - 1), r);
+        const int all_lo = __builtin_amdgcn_readfirstlane(wr.all_lo), all_hi = __builtin_amdgcn_readfirstlane(wr.all_hi);
         if (lane == 0) {
-            s_lo[i][wave] = own_lo;
-            s_hi[i][wave] = own_hi;
+            s_lo[i][wave] = wr.lo;
+            s_hi[i][wave] = wr.hi;
         }
         __syncthreads();
         int lo = min(min(s_lo[i][0], s_lo[i][1]), min(s_lo[i][2], s_lo[i][3]));
@@ -747,9 +775,9 @@ __global__ void __launch_bounds__(256, 2) attn_keys_kernel(const MaskArgs a, con
         const KeySpan& sp = job.span[i];
         const Range r = row_range(a, job.kind[i], sp, rp);
         live = r.live;
-        const bool some = r.hi > r.lo;
-        int lo = wave_min(some ? r.lo : 0x7fffffff), hi = wave_max(some ? r.hi : 0);
-        const int all_lo = wave_max(r.lo), all_hi = wave_min(r.hi); // what every row sees
+        const WaveRange wr = wave_range(a, job, job.kind[i], sp, it.seq, row0, min(row0 + 31, job.rows - 1), r);
+        const int all_lo = __builtin_amdgcn_readfirstlane(wr.all_lo), all_hi = __builtin_amdgcn_readfirstlane(wr.all_hi);
+        int lo = __builtin_amdgcn_readfirstlane(wr.lo), hi = __builtin_amdgcn_readfirstlane(wr.hi);
         int nb = hi > lo ? (hi - lo + KB - 1) / KB : 0;
         if (job.splits > 1) {
             const int per = (nb + job.splits - 1) / job.splits;
@@ -888,20 +916,33 @@ __global__ void __launch_bounds__(256, 2) attn_keys_kernel(const MaskArgs a, con
     rows_alone<F16, MODE>(a, to, s_bad & (0x11111111u << wave), row0, 0, first, end, slope, lane); // (every wave a quarter of them)
 }
 
-// The shares of each row's keys, joined in their order: half a wave a row.
-template <bool F16>
+// The shares of each row's keys, joined: WAYS half waves take a row's parts in turn, four at a time, and their sums are
+// joined in their order. Bound by the parts' way to memory and back; one half wave for all parts of a row took 12.6 us for 128
+// rows of 16 parts.
+template <bool F16, int WAYS>
 __global__ void __launch_bounds__(256) attn_masked_merge_kernel(const MaskArgs a, int rows) {
-    const int r = (int)blockIdx.x * 8 + ((int)threadIdx.x >> 5); // (sequence, key head, row of the sequence)
-    const int c = (int)threadIdx.x & 31;
-    if (r >= rows) return;
+    constexpr int ROWS = 8 / WAYS; // of a workgroup
+    __shared__ float s_o[WAYS == 1 ? 1 : 8][D], s_ml[8][2];
+    const int hw = (int)threadIdx.x >> 5, c = (int)threadIdx.x & 31;
+    const int way = hw % WAYS;
+    const int r = min((int)blockIdx.x * ROWS + hw / WAYS, rows - 1); // (sequence, key head, row of the sequence)
+    const bool mine = (int)blockIdx.x * ROWS + hw / WAYS < rows;
     const int per = a.q_tokens * a.group;
     const int sk = r / per;
     const int rr = r - sk * per;
     const int kvh = sk % a.kv_heads, seq = sk / a.kv_heads;
     const RowPos p{seq, rr / a.group, rr % a.group};
-    if (!row_range(a, a.job[0].kind[0], a.job[0].span[0], p).live) return;
     float m = -INFINITY, l = 0.f;
     f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto add = [&](float ms, float ls, const f32x4& x) __attribute__((always_inline)) {
+        if (ls == 0.f) return; // (a part without keys: x was never written)
+        const float top = fmaxf(m, ms); // (a NaN is in l and o by then)
+        const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top), g = __builtin_amdgcn_exp2f(ms - top);
+        l = l * f + ls * g;
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[j] = o[j] * f + x[j] * g;
+        m = top;
+    };
     for (int n = 0; n < a.jobs; n++) {
         const MaskJob& job = a.job[n];
         const int tr = job.by_keys ? kMaskRowsByKeys : kMaskRowsByWave;
@@ -909,20 +950,35 @@ __global__ void __launch_bounds__(256) attn_masked_merge_kernel(const MaskArgs a
         const int at_sk = job.pooled ? kvh : sk;
         const int tile = row / tr;
         const int64_t at = job.part_base + (int64_t)(at_sk * job.row_tiles + tile) * job.splits * tr + (row - tile * tr);
-#pragma clang loop unroll_count(4)
-        for (int s = 0; s < job.splits; s++) {
-            const int64_t i = at + (int64_t)s * tr;
-            const float ms = a.part_ml[2 * i], ls = a.part_ml[2 * i + 1];
-            if (ls == 0.f) continue;
-            const f32x4 x = *reinterpret_cast<const f32x4*>(a.part_o + i * D + 4 * c);
-            const float top = fmaxf(m, ms); // (a NaN is in l and o by then)
-            const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top), g = __builtin_amdgcn_exp2f(ms - top);
-            l = l * f + ls * g;
+        for (int s = way; s < job.splits; s += 4 * WAYS) {
+            float ml[4][2];
+            f32x4 x[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) o[j] = o[j] * f + x[j] * g;
-            m = top;
+            for (int u = 0; u < 4; u++) {
+                const int64_t i = at + (int64_t)min(s + u * WAYS, job.splits - 1) * tr;
+                ml[u][0] = a.part_ml[2 * i];
+                ml[u][1] = s + u * WAYS < job.splits ? a.part_ml[2 * i + 1] : 0.f;
+                x[u] = *reinterpret_cast<const f32x4*>(a.part_o + i * D + 4 * c);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++) add(ml[u][0], ml[u][1], x[u]);
         }
     }
+    if constexpr (WAYS > 1) {
+        *reinterpret_cast<f32x4*>(&s_o[hw][4 * c]) = o;
+        if (c == 0) {
+            s_ml[hw][0] = m;
+            s_ml[hw][1] = l;
+        }
+        __syncthreads();
+        if (way != 0) return;
+        m = -INFINITY;
+        l = 0.f;
+        o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < WAYS; w++) add(s_ml[hw + w][0], s_ml[hw + w][1], *reinterpret_cast<const f32x4*>(&s_o[hw + w][4 * c]));
+    }
+    if (!mine || !row_range(a, a.job[0].kind[0], a.job[0].span[0], p).live) return;
     const float inv = l == 0.f ? 0.f : 1.0f / l;
     char* const out = a.o + (int64_t)seq * a.o_ss + (int64_t)p.tok * a.o_ts + (int64_t)(kvh * a.group + p.g) * a.o_hs;
     *reinterpret_cast<u32x2*>(out + 8 * c) = u32x2{round2<F16>(o[0] * inv, o[1] * inv), round2<F16>(o[2] * inv, o[3] * inv)};
@@ -954,7 +1010,10 @@ hipError_t launch_typed(const MaskArgs& a, hipStream_t stream) {
     if (e != hipSuccess || a.direct) return e;
     const MaskJob& last = a.job[a.jobs - 1]; // tiled by sequence
     const int rows = last.seqs * a.kv_heads * last.rows;
-    msk::attn_masked_merge_kernel<F16><<<dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, stream>>>(a, rows);
+    int parts = 0;
+    for (int i = 0; i < a.jobs; i++) parts += a.job[i].splits;
+    if (parts > 4) msk::attn_masked_merge_kernel<F16, 8><<<dim3((unsigned)rows), dim3(256), 0, stream>>>(a, rows);
+    else msk::attn_masked_merge_kernel<F16, 1><<<dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, stream>>>(a, rows);
     return hipGetLastError();
 }
 
