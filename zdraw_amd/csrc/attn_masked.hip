@@ -60,6 +60,15 @@ struct RowPos {
     int seq, tok, g;
 };
 
+// x / d for 0 <= x < 2^24: exact in f32 but for one, which the remainder tells.
+__device__ __forceinline__ int div24(int x, int d) {
+    int q = (int)((float)x * __builtin_amdgcn_rcpf((float)d));
+    const int r = x - q * d;
+    q += r >= d ? 1 : 0;
+    q -= r < 0 ? 1 : 0;
+    return q;
+}
+
 // The keys a row sees, in its span's own numbering, and where it stands among them.
 struct Range {
     int lo, hi, pos;
@@ -68,10 +77,10 @@ struct Range {
 
 __device__ __forceinline__ RowPos row_pos(const MaskArgs& a, const MaskJob& job, int seq, int r) {
     RowPos p;
-    const int t = r / a.group;
+    const int t = div24(r, a.group);
     p.g = r - t * a.group;
     if (job.pooled) {
-        p.seq = t / a.q_tokens;
+        p.seq = div24(t, a.q_tokens);
         p.tok = t - p.seq * a.q_tokens;
     } else {
         p.seq = seq;
@@ -112,7 +121,8 @@ __device__ __forceinline__ Range row_range(const MaskArgs& a, int kind, const Ke
         r.hi = ks + n;
         r.pos = ks + at;
     } else {
-        const int n = a.lens ? (int)min(a.lens[p.seq], (unsigned)a.own_keys) : 0;
+        // (of the prefix, what a request holds itself counts for the bias alone)
+        const int n = a.lens && (kind != kRangePrefix || a.slopes) ? (int)min(a.lens[p.seq], (unsigned)a.own_keys) : 0;
         const int ql = a.q_lens ? (int)min(a.q_lens[p.seq], (unsigned)a.q_tokens) : a.q_tokens;
         r.live = p.tok < ql;
         const int at = p.tok + n - ql;
@@ -132,6 +142,7 @@ __device__ __forceinline__ Range row_range(const MaskArgs& a, int kind, const Ke
 // `last_row`: of the wave's rows, held to the sequence. Without documents the ranges of a sequence's rows only grow.
 struct WaveRange {
     int lo, hi, all_lo, all_hi;
+    int pos_lo, pos_hi; // where the first and the last row stand
 };
 __device__ __forceinline__ int wave_min(int x);
 __device__ __forceinline__ int wave_max(int x);
@@ -143,17 +154,22 @@ __device__ __forceinline__ WaveRange wave_range(const MaskArgs& a, const MaskJob
         w.hi = wave_max(some ? r.hi : 0);
         w.all_lo = wave_max(r.lo);
         w.all_hi = wave_min(r.hi);
+        w.pos_lo = wave_min(r.pos);
+        w.pos_hi = wave_max(r.pos);
         return w;
     }
     w.lo = w.all_lo = 0;
-    if (kind == kRangePrefix) {
-        // (rows past their request's are among those that "see" the prefix: they are not written)
+    if (job.pooled) { // (the prefix)
         w.hi = w.all_hi = sp.keys;
+        w.pos_lo = a.slopes ? wave_min(r.pos) : 0;
+        w.pos_hi = a.slopes ? wave_max(r.pos) : 0;
         return w;
     }
-    const Range lo = row_range(a, kind, sp, RowPos{seq, first_row / a.group, 0}), hi = row_range(a, kind, sp, RowPos{seq, last_row / a.group, 0});
+    const Range lo = row_range(a, kind, sp, RowPos{seq, div24(first_row, a.group), 0}), hi = row_range(a, kind, sp, RowPos{seq, div24(last_row, a.group), 0});
     w.all_hi = hi.live ? lo.hi : 0;
     w.hi = hi.live ? hi.hi : wave_max(r.hi);
+    w.pos_lo = lo.pos;
+    w.pos_hi = hi.pos;
     return w;
 }
 
@@ -223,6 +239,36 @@ __device__ __forceinline__ void load_rows(const KeySpan& sp, const SpanBase& b, 
     else rows_to_lds(kp, q * (unsigned)sp.k_ts + k_chunk(lane, n), lds + (unsigned)n * 1024u);
 }
 
+// A block of K or V, eight loads: rows j .. j + 31, of which those past `last` repeat it. Rows that lie apart by one stride take
+// their places from it; on pages a run of rows that one page holds is looked up at a time.
+template <bool V>
+__device__ __forceinline__ void load_block(const KeySpan& sp, const SpanBase& b, int lane, const unsigned (&off)[4], int j, int last, unsigned lds) {
+    const unsigned ts = (unsigned)(V ? sp.v_ts : sp.k_ts);
+    if (!sp.table && j + KB - 1 <= last) {
+        const char* p = V ? b.v + (int64_t)j * ts : b.k + (int64_t)j * ts;
+#pragma unroll
+        for (int n = 0; n < 8; n++) {
+            rows_to_lds(p, off[V ? 0 : n & 3], lds + (unsigned)n * 1024u);
+            p += 4 * (int64_t)ts;
+        }
+        return;
+    }
+    const int run = sp.table ? min(sp.page_mask + 1, KB) : KB;
+#pragma clang loop unroll(disable)
+    for (int r0 = 0; r0 < KB; r0 += run) {
+        const int jr = min(j + r0, last);
+        const char *kp, *vp;
+        row_at(sp, b, jr, kp, vp);
+        const int left = last - jr;
+#pragma clang loop unroll(disable)
+        for (int x = 0; x < run; x += 4) {
+            const int n = (r0 + x) >> 2;
+            const unsigned row = (unsigned)min(lane >> 4, max(left - x, 0)); // (of four: 32 bits hold its offset)
+            rows_to_lds((V ? vp : kp) + (int64_t)min(x, left) * ts, row * ts + (V ? v_chunk(lane) : k_chunk(lane, n)), lds + (unsigned)n * 1024u);
+        }
+    }
+}
+
 // What a lane keeps of its row across the key blocks. O^T: lane row l32, dims 32 b + 8 i + 4 h + j in o[b][4 i + j].
 struct RowState {
     f32x16 o[4];
@@ -247,19 +293,66 @@ __device__ __forceinline__ bf16x8 round8(const T& p, int at) {
 // What becomes of a product q.k before the softmax.
 enum ScoreMode : int { kPlain = 0, kBias = 1, kCap = 2 }; // kCap: and biased, by a slope that may be 0
 
-// A score of one key, log2, where it is more than a scaled product (kPlain: the scale is in the exponential's fma).
+// A capped score, log2: cap tanh(s / cap). tanh x = 1 - 2 / (e^2x + 1) is 1 and -1 at the infinities and NaN at NaN; near 0 it is
+// off by 2^-24 of the cap.
+__device__ __forceinline__ float capped(const MaskArgs& a, float dot) {
+    return __builtin_fmaf(-2.0f * a.cap_out, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(dot * a.cap_in) + 1.0f), a.cap_out);
+}
+// A score of one key by itself, log2.
 template <int MODE>
 __device__ __forceinline__ float score_of(const MaskArgs& a, float dot, float slope, float dist) {
-    // cap tanh(s / cap): tanh x = 1 - 2 / (e^2x + 1) is 1 and -1 at the infinities and NaN at NaN; near 0 it is off by 2^-24 of the cap
-    const float y = MODE == kCap ? __builtin_fmaf(-2.0f * a.cap_out, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(dot * a.cap_in) + 1.0f), a.cap_out) : dot * a.scale_log2;
-    return __builtin_fmaf(-slope, fabsf(dist), y);
+    const float y = MODE == kCap ? capped(a, dot) : dot * a.scale_log2;
+    return MODE == kPlain ? y : __builtin_fmaf(-slope, fabsf(dist), y);
+}
+
+// The bias over a block of keys. From the row's place on one side of the block its distance is linear in the key, and
+// the bias is one fma beside the scale's: key x of the lane gets at + x step. Where the row stands inside the block the scores
+// are first bent (bend_block) so that the same line fits.
+struct BiasLine {
+    float step, at;
+};
+struct RowBias {
+    float slope;      // log2(e) x the head's; 0 without a bias
+    int pos;          // where the row stands
+    int pos_lo, pos_hi; // of all rows of the wave
+    bool ahead;       // no row sees a key behind itself
+};
+template <int MODE>
+__device__ __forceinline__ BiasLine bias_line(const RowBias& rb, int j0, int h) {
+    BiasLine line{0.f, 0.f};
+    if constexpr (MODE != kPlain) {
+        line.step = !rb.ahead && j0 >= rb.pos_hi ? -rb.slope : rb.slope;
+        line.at = -line.step * (float)(rb.pos - j0 - 4 * h);
+    }
+    return line;
+}
+// A biased row's scores rise towards where it stands (`pos`, the last of the rows'): its blocks are walked from there, down and then up, so that the
+// reference point is found at once and not moved by every block (16384 causal tokens, 24 heads: 2586 us first to last).
+template <int MODE>
+__device__ __forceinline__ int blocks_down(const MaskArgs& a, int pos, int lo, int nb) {
+    if (MODE == kPlain || !a.slopes || pos < lo) return 0;
+    return min((pos - lo) / KB + 1, nb);
+}
+__device__ __forceinline__ void bend_block(const RowBias& rb, f32x16& s, float c, int j0, int h) {
+    const float k = 2.0f * rb.slope / c, d0 = (float)(rb.pos - j0 - 4 * h);
+#pragma unroll
+    for (int i = 0; i < 16; i++) s[i] = __builtin_fmaf(k, fminf(d0 - (float)(8 * (i >> 2) + (i & 3)), 0.0f), s[i]); // -|d| = -d + 2 min(d, 0)
 }
 template <int MODE>
-__device__ __forceinline__ void score_block(const MaskArgs& a, f32x16& s, int j0, int h, int pos, float slope) {
-    if constexpr (MODE != kPlain) {
-        const float d0 = (float)(pos - j0 - 4 * h);
+__device__ __forceinline__ float scaled(float s, float c, const BiasLine& line, int i) {
+    if constexpr (MODE == kPlain) return __builtin_fmaf(s, c, line.at);
+    else return __builtin_fmaf(s, c, __builtin_fmaf(line.step, (float)(8 * (i >> 2) + (i & 3)), line.at));
+}
+
+// The cap, the bend of the bias and the mask of a block's products. Most blocks of most calls need none of it.
+template <int MODE>
+__device__ __forceinline__ void finish_block(const MaskArgs& a, f32x16& s, float c, const RowBias& rb, int j0, int h) {
+    if constexpr (MODE == kCap) {
 #pragma unroll
-        for (int i = 0; i < 16; i++) s[i] = score_of<MODE>(a, s[i], slope, d0 - (float)(8 * (i >> 2) + (i & 3)));
+        for (int i = 0; i < 16; i++) s[i] = capped(a, s[i]);
+    }
+    if constexpr (MODE != kPlain) {
+        if (!rb.ahead && j0 + KB - 1 > rb.pos_lo && j0 < rb.pos_hi) bend_block(rb, s, c, j0, h);
     }
 }
 __device__ __forceinline__ void mask_block(f32x16& s, int j0, int h, const Range& r) {
@@ -268,18 +361,25 @@ __device__ __forceinline__ void mask_block(f32x16& s, int j0, int h, const Range
 #pragma unroll
     for (int i = 0; i < 16; i++) s[i] = first + (unsigned)(8 * (i >> 2) + (i & 3)) < n ? s[i] : -INFINITY;
 }
-__device__ __forceinline__ float block_max(const f32x16& s) {
-    float top = fmaxf(s[0], s[1]);
+template <int MODE>
+__device__ __forceinline__ float block_max(const f32x16& s, float c, const BiasLine& line) {
+    if constexpr (MODE == kPlain) {
+        float top = fmaxf(s[0], s[1]);
 #pragma unroll
-    for (int i = 2; i < 16; i += 2) top = fmaxf(top, fmaxf(s[i], s[i + 1]));
-    return pair_max(top);
+        for (int i = 2; i < 16; i += 2) top = fmaxf(top, fmaxf(s[i], s[i + 1]));
+        return pair_max(top) * c;
+    } else {
+        float top = scaled<MODE>(s[0], c, line, 0);
+#pragma unroll
+        for (int i = 1; i < 16; i++) top = fmaxf(top, scaled<MODE>(s[i], c, line, i));
+        return pair_max(top);
+    }
 }
 
 // Scores of a block -> P (16 bits), with the row's reference point, denominator and O kept up.
 template <bool F16, int MODE>
-__device__ __forceinline__ void softmax_block(const MaskArgs& a, f32x16& s, RowState& st, bf16x8 (&p)[2]) {
-    const float c = MODE == kPlain ? a.scale_log2 : 1.0f;
-    const float top = block_max(s) * c;
+__device__ __forceinline__ void softmax_block(const f32x16& s, float c, const BiasLine& line, RowState& st, bf16x8 (&p)[2]) {
+    const float top = block_max<MODE>(s, c, line);
     const bool move = top > st.m + kTau; // (from -infinity: any score)
     if (__builtin_amdgcn_ballot_w64(move) != 0) {
         const float m = move ? top : st.m;
@@ -291,16 +391,16 @@ __device__ __forceinline__ void softmax_block(const MaskArgs& a, f32x16& s, RowS
 #pragma unroll
             for (int i = 0; i < 16; i++) st.o[b][i] *= f;
     }
-    const float ref = st.m == -INFINITY ? 0.0f : st.m;
-    float sum = 0.f;
+    const BiasLine down{line.step, line.at - (st.m == -INFINITY ? 0.0f : st.m)};
+    float sum = 0.f, e[16];
 #pragma unroll
     for (int i = 0; i < 16; i++) {
-        s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -ref));
-        sum += s[i];
+        e[i] = __builtin_amdgcn_exp2f(scaled<MODE>(s[i], c, down, i));
+        sum += e[i];
     }
     st.l += sum;
-    p[0] = round8<F16>(s, 0);
-    p[1] = round8<F16>(s, 8);
+    p[0] = round8<F16>(e, 0);
+    p[1] = round8<F16>(e, 8);
 }
 
 struct FragLane {
@@ -344,7 +444,7 @@ __device__ void row_alone(const MaskArgs& a, const KeySpan& sp, const SpanBase& 
         float s = q0 * k0 + q1 * k1;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o);
-        s = MODE == kPlain ? s * a.scale_log2 : score_of<MODE>(a, s, slope, (float)(pos - j));
+        s = score_of<MODE>(a, s, slope, (float)(pos - j));
         if (!(s <= m)) { // (a NaN moves the reference to NaN, and stays)
             const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - s);
             m = s;
@@ -381,12 +481,17 @@ __device__ __forceinline__ Item item_of(const MaskArgs& a, const MaskJob& job, i
     const int xcd = id & 7, idx = id >> 3, per = job.workgroups >> 3, rem = job.workgroups & 7;
     const int item = idx + xcd * per + min(xcd, rem);
     Item it;
-    it.tile = job.row_tiles - 1 - item % job.row_tiles; // the last rows see the most keys: first
-    const int rest = item / job.row_tiles;
-    it.split = rest % job.splits;
-    it.sk = rest / job.splits;
-    it.kvh = it.sk % a.kv_heads;
-    it.seq = it.sk / a.kv_heads;
+    const int rest = div24(item, job.row_tiles);
+    it.tile = job.row_tiles - 1 - (item - rest * job.row_tiles); // the last rows see the most keys: first
+    it.sk = div24(rest, job.splits);
+    it.split = rest - it.sk * job.splits;
+    it.seq = div24(it.sk, a.kv_heads);
+    it.kvh = it.sk - it.seq * a.kv_heads;
+    it.tile = __builtin_amdgcn_readfirstlane(it.tile);
+    it.sk = __builtin_amdgcn_readfirstlane(it.sk);
+    it.split = __builtin_amdgcn_readfirstlane(it.split);
+    it.seq = __builtin_amdgcn_readfirstlane(it.seq);
+    it.kvh = __builtin_amdgcn_readfirstlane(it.kvh);
     return it;
 }
 
@@ -459,8 +564,9 @@ __device__ __forceinline__ void lane_offsets(int lane, FragLane& fl) {
 // A reference point that moves in step b rescales O at its end: what P(b - 1) adds in it still goes by the old one.
 template <bool F16, int MODE>
 __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, const int which) {
+    touch_args<sizeof(MaskArgs) + sizeof(int)>();
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    __shared__ int s_lo[2][4], s_hi[2][4];
+    __shared__ int s_lo[2][4], s_hi[2][4], s_pos[2][4];
     constexpr unsigned kV = kStages * kBlock; // the V ring behind the K ring
 
     const int tid = threadIdx.x;
@@ -477,7 +583,7 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
     const RowPos rp = row_pos(a, job, it.seq, row);
     const int head = it.kvh * a.group + rp.g;
     const float slope = (MODE != kPlain && a.slopes) ? a.slopes[head] * 1.4426950408889634f : 0.0f;
-    const float c = MODE == kPlain ? a.scale_log2 : 1.0f;
+    const float c = MODE == kCap ? 1.0f : a.scale_log2;
 
     const char* const qrow = a.q + (int64_t)rp.seq * a.q_ss + (int64_t)rp.tok * a.q_ts + (int64_t)head * a.q_hs;
     bf16x8 qf[8];
@@ -507,9 +613,12 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
         live = r.live;
         const WaveRange wr = wave_range(a, job, job.kind[i], sp, it.seq, min(row0, job.rows - 1), min(row0 + 31, job.rows - 1), r);
         const int all_lo = __builtin_amdgcn_readfirstlane(wr.all_lo), all_hi = __builtin_amdgcn_readfirstlane(wr.all_hi);
+        const RowBias rb{slope, r.pos, __builtin_amdgcn_readfirstlane(wr.pos_lo), __builtin_amdgcn_readfirstlane(wr.pos_hi),
+                         a.causal && !a.prefix && job.kind[i] != kRangePrefix};
         if (lane == 0) {
             s_lo[i][wave] = wr.lo;
             s_hi[i][wave] = wr.hi;
+            s_pos[i][wave] = wr.pos_hi;
         }
         __syncthreads();
         int lo = min(min(s_lo[i][0], s_lo[i][1]), min(s_lo[i][2], s_lo[i][3]));
@@ -537,33 +646,34 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
         const unsigned lq = (unsigned)lane >> 4;
         const unsigned ko0 = lq * (unsigned)sp.k_ts + k_chunk(lane, 2 * wave), ko1 = (lq + 4) * (unsigned)sp.k_ts + k_chunk(lane, 2 * wave + 1);
         const unsigned vo0 = lq * (unsigned)sp.v_ts + v_chunk(lane), vo1 = vo0 + 4 * (unsigned)sp.v_ts;
-        const int whole_blocks = base.table ? 0 : (hi - lo) / KB; // those that lie in memory as they do in LDS
-        const char* kp = base.k + (int64_t)(lo + 8 * wave) * sp.k_ts;
-        const char* vp = base.v + (int64_t)(lo + 8 * wave) * sp.v_ts;
-        const int64_t k_step = (int64_t)KB * sp.k_ts, v_step = (int64_t)KB * sp.v_ts;
+        const int whole_end = base.table ? 0 : lo + (hi - lo) / KB * KB; // up to here blocks lie in memory as they do in LDS
+        const int n_down = blocks_down<MODE>(a, __builtin_amdgcn_readfirstlane(max(max(s_pos[i][0], s_pos[i][1]), max(s_pos[i][2], s_pos[i][3]))), lo, nb);
+        auto first_key = [&](int b) __attribute__((always_inline)) { return lo + (b < n_down ? n_down - 1 - b : b) * KB; };
         const unsigned lds_w = lds0 + (unsigned)wave * 2048u;
         auto fetch_k = [&](int b) __attribute__((always_inline)) {
             const unsigned at = lds_w + (unsigned)(b & (kStages - 1)) * (unsigned)kBlock;
-            if (b < whole_blocks) {
-                rows_to_lds(kp, ko0, at);
-                rows_to_lds(kp, ko1, at + 1024u);
-                kp += k_step;
+            const int j = first_key(b);
+            if (j < whole_end) {
+                const char* const p = base.k + (int64_t)(j + 8 * wave) * sp.k_ts;
+                rows_to_lds(p, ko0, at);
+                rows_to_lds(p, ko1, at + 1024u);
             } else {
                 const int ln = lane_again();
-                load_rows<false>(sp, base, ln, lo + b * KB + 8 * wave, last, 2 * wave, at - (unsigned)wave * 2048u);
-                load_rows<false>(sp, base, ln, lo + b * KB + 8 * wave + 4, last, 2 * wave + 1, at - (unsigned)wave * 2048u);
+                load_rows<false>(sp, base, ln, j + 8 * wave, last, 2 * wave, at - (unsigned)wave * 2048u);
+                load_rows<false>(sp, base, ln, j + 8 * wave + 4, last, 2 * wave + 1, at - (unsigned)wave * 2048u);
             }
         };
         auto fetch_v = [&](int b) __attribute__((always_inline)) {
             const unsigned at = lds_w + kV + (unsigned)(b & (kStages - 1)) * (unsigned)kBlock;
-            if (b < whole_blocks) {
-                rows_to_lds(vp, vo0, at);
-                rows_to_lds(vp, vo1, at + 1024u);
-                vp += v_step;
+            const int j = first_key(b);
+            if (j < whole_end) {
+                const char* const p = base.v + (int64_t)(j + 8 * wave) * sp.v_ts;
+                rows_to_lds(p, vo0, at);
+                rows_to_lds(p, vo1, at + 1024u);
             } else {
                 const int ln = lane_again();
-                load_rows<true>(sp, base, ln, lo + b * KB + 8 * wave, last, 2 * wave, at - (unsigned)wave * 2048u);
-                load_rows<true>(sp, base, ln, lo + b * KB + 8 * wave + 4, last, 2 * wave + 1, at - (unsigned)wave * 2048u);
+                load_rows<true>(sp, base, ln, j + 8 * wave, last, 2 * wave, at - (unsigned)wave * 2048u);
+                load_rows<true>(sp, base, ln, j + 8 * wave + 4, last, 2 * wave + 1, at - (unsigned)wave * 2048u);
             }
         };
         // P(-1) = 0 meets the V stage of "block -1", which has to hold finite numbers
@@ -583,13 +693,13 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
         for (int t = 0; t < 8; t++) s_a = mfma<F16>(k_frag(0, fl, t), qf[t], s_a);
         p_a[0] = p_a[1] = __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u});
         auto finish_scores = [&](f32x16& s, int b) __attribute__((always_inline)) {
-            const int j0 = lo + b * KB;
-            score_block<MODE>(a, s, j0, h, r.pos, slope);
+            const int j0 = first_key(b);
+            finish_block<MODE>(a, s, c, rb, j0, h);
             if (!(j0 >= all_lo && j0 + KB <= all_hi)) mask_block(s, j0, h, r);
         };
         // The reference point at a block's maximum, where that is higher: what was summed goes by the new one.
-        auto raise = [&](const f32x16& s) __attribute__((always_inline)) {
-            const float m = fmaxf(st.m, block_max(s) * c);
+        auto raise = [&](const f32x16& s, int b) __attribute__((always_inline)) {
+            const float m = fmaxf(st.m, block_max<MODE>(s, c, bias_line<MODE>(rb, first_key(b), h)));
             const float f = st.m == m ? 1.0f : __builtin_amdgcn_exp2f(st.m - m);
             st.m = m;
             st.l *= f;
@@ -599,7 +709,7 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
                 for (int j = 0; j < 16; j++) st.o[d][j] *= f;
         };
         finish_scores(s_a, 0);
-        raise(s_a);
+        raise(s_a, 0);
 
         auto step = [&](auto phase, int b, f32x16& s, f32x16& s_next, const bf16x8 (&p_old)[2], bf16x8 (&p)[2]) __attribute__((always_inline)) {
             constexpr int J = decltype(phase)::value;
@@ -621,7 +731,9 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
             };
 #pragma unroll
             for (int x = 0; x < LA; x++) read(x);
-            const float ref = st.m == -INFINITY ? 0.0f : st.m;
+            const int j0 = first_key(b);
+            BiasLine line = bias_line<MODE>(rb, j0, h);
+            line.at -= st.m == -INFINITY ? 0.0f : st.m;
             float sum = 0.f, e[16];
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -629,7 +741,7 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
                 if (x + LA < 16) read(x + LA);
                 if (x & 1) st.o[(x >> 1) & 3] = mfma<F16>(__builtin_bit_cast(bf16x8, vf[x >> 1]), p_old[x >> 3], st.o[(x >> 1) & 3]);
                 else s_next = mfma<F16>(kf[x >> 1], qf[x >> 1], x == 0 ? zero : s_next);
-                e[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x], c, -ref));
+                e[x] = __builtin_amdgcn_exp2f(scaled<MODE>(s[x], c, line, x));
                 sum += e[x];
                 pin(sum);
                 if ((x & 7) == 7) {
@@ -639,14 +751,14 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
                 __builtin_amdgcn_sched_barrier(0);
             }
             // a score far above the reference point, a number that is none, or the first block that a row sees
-            const int j0 = lo + b * KB;
             if (__builtin_amdgcn_ballot_w64(!(sum <= kLimit) || (st.m == -INFINITY && r.lo < j0 + KB && r.hi > j0)) != 0) {
-                raise(s);
-                const float ref2 = st.m == -INFINITY ? 0.0f : st.m;
+                raise(s, b);
+                line = bias_line<MODE>(rb, j0, h);
+                line.at -= st.m == -INFINITY ? 0.0f : st.m;
                 sum = 0.f;
 #pragma unroll
                 for (int x = 0; x < 16; x++) {
-                    e[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x], c, -ref2));
+                    e[x] = __builtin_amdgcn_exp2f(scaled<MODE>(s[x], c, line, x));
                     sum += e[x];
                 }
                 p[0] = round8<F16>(e, 0);
@@ -732,6 +844,7 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
 // one's fragments are in registers, V likewise, so that 8 to 16 KB a wave, eight waves a CU, are always on their way.
 template <bool F16, int MODE>
 __global__ void __launch_bounds__(256, 2) attn_keys_kernel(const MaskArgs a, const int which0) {
+    touch_args<sizeof(MaskArgs) + sizeof(int)>();
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     __shared__ float s_ml[4][KB][2];
     __shared__ unsigned s_bad;
@@ -752,6 +865,7 @@ __global__ void __launch_bounds__(256, 2) attn_keys_kernel(const MaskArgs a, con
     const RowPos rp = row_pos(a, job, it.seq, row);
     const int head = it.kvh * a.group + rp.g;
     const float slope = (MODE != kPlain && a.slopes) ? a.slopes[head] * 1.4426950408889634f : 0.0f;
+    const float c = MODE == kCap ? 1.0f : a.scale_log2;
 
     const char* const qrow = a.q + (int64_t)rp.seq * a.q_ss + (int64_t)rp.tok * a.q_ts + (int64_t)head * a.q_hs;
     bf16x8 qf[8];
@@ -777,6 +891,8 @@ __global__ void __launch_bounds__(256, 2) attn_keys_kernel(const MaskArgs a, con
         live = r.live;
         const WaveRange wr = wave_range(a, job, job.kind[i], sp, it.seq, row0, min(row0 + 31, job.rows - 1), r);
         const int all_lo = __builtin_amdgcn_readfirstlane(wr.all_lo), all_hi = __builtin_amdgcn_readfirstlane(wr.all_hi);
+        const RowBias rb{slope, r.pos, __builtin_amdgcn_readfirstlane(wr.pos_lo), __builtin_amdgcn_readfirstlane(wr.pos_hi),
+                         a.causal && !a.prefix && job.kind[i] != kRangePrefix};
         int lo = __builtin_amdgcn_readfirstlane(wr.lo), hi = __builtin_amdgcn_readfirstlane(wr.hi);
         int nb = hi > lo ? (hi - lo + KB - 1) / KB : 0;
         if (job.splits > 1) {
@@ -796,34 +912,38 @@ __global__ void __launch_bounds__(256, 2) attn_keys_kernel(const MaskArgs a, con
         const int last = hi - 1;
         const SpanBase base = span_base(sp, it.seq, it.kvh);
         const unsigned kl = lds0 + (unsigned)wave * (2u * kBlock), vl = kl + kBlock;
+        const unsigned k_off0 = ((unsigned)lane >> 4) * (unsigned)sp.k_ts, v_off0 = ((unsigned)lane >> 4) * (unsigned)sp.v_ts;
+        const unsigned k_off[4] = {k_off0 + k_chunk(lane, 0), k_off0 + k_chunk(lane, 1), k_off0 + k_chunk(lane, 2), k_off0 + k_chunk(lane, 3)};
+        const unsigned v_off[4] = {v_off0 + v_chunk(lane), 0u, 0u, 0u};
+        const int n_down = blocks_down<MODE>(a, rb.pos_hi, lo, nb);
+        auto first_key = [&](int b) __attribute__((always_inline)) { return lo + (b < n_down ? n_down - 1 - b : b) * KB; };
         if (wave < nb) {
-#pragma unroll
-            for (int n = 0; n < 8; n++) load_rows<false>(sp, base, lane, lo + wave * KB + 4 * n, last, n, kl);
-#pragma unroll
-            for (int n = 0; n < 8; n++) load_rows<true>(sp, base, lane, lo + wave * KB + 4 * n, last, n, vl);
+            load_block<false>(sp, base, lane, k_off, first_key(wave), last, kl);
+            load_block<true>(sp, base, lane, v_off, first_key(wave), last, vl);
         }
+        // (The query rows are here before the loop: the compiler, which does not know of the loads above, would wait for all
+        // loads at their first use in it, every time around: three drafts of 7 requests over a 30011-key prefix 35.8 us.)
+#pragma unroll
+        for (int t = 0; t < 8; t++) pin(qf[t]);
 #pragma clang loop unroll(disable)
         for (int b = wave; b < nb; b += 4) {
             const bool more = b + 4 < nb;
-            const int j0 = lo + b * KB;
+            const int j0 = first_key(b), j_next = first_key(b + 4);
             wait_loads<8>(); // K has arrived, V may be on its way
             bf16x8 kf[8];
 #pragma unroll
             for (int t = 0; t < 8; t++) kf[t] = k_frag(kl, fl, t);
             asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-            if (more) {
-#pragma unroll
-                for (int n = 0; n < 8; n++) load_rows<false>(sp, base, lane, j0 + 4 * KB + 4 * n, last, n, kl);
-            }
+            if (more) load_block<false>(sp, base, lane, k_off, j_next, last, kl);
             f32x16 s;
 #pragma unroll
             for (int j = 0; j < 16; j++) s[j] = 0.f;
 #pragma unroll
             for (int t = 0; t < 8; t++) s = mfma<F16>(kf[t], qf[t], s);
-            score_block<MODE>(a, s, j0, h, r.pos, slope);
+            finish_block<MODE>(a, s, c, rb, j0, h);
             if (!(j0 >= all_lo && j0 + KB <= all_hi)) mask_block(s, j0, h, r);
             bf16x8 p[2];
-            softmax_block<F16, MODE>(a, s, st, p);
+            softmax_block<F16, MODE>(s, c, bias_line<MODE>(rb, j0, h), st, p);
             if (more) wait_loads<8>();
             else wait_loads<0>();
             s16x8 vf[2][4];
@@ -832,10 +952,7 @@ __global__ void __launch_bounds__(256, 2) attn_keys_kernel(const MaskArgs a, con
 #pragma unroll
                 for (int d = 0; d < 4; d++) vf[kb][d] = v_frag(vl, fl, kb, d);
             asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-            if (more) {
-#pragma unroll
-                for (int n = 0; n < 8; n++) load_rows<true>(sp, base, lane, j0 + 4 * KB + 4 * n, last, n, vl);
-            }
+            if (more) load_block<true>(sp, base, lane, v_off, j_next, last, vl);
 #pragma unroll
             for (int kb = 0; kb < 2; kb++)
 #pragma unroll
@@ -921,6 +1038,7 @@ __global__ void __launch_bounds__(256, 2) attn_keys_kernel(const MaskArgs a, con
 // rows of 16 parts.
 template <bool F16, int WAYS>
 __global__ void __launch_bounds__(256) attn_masked_merge_kernel(const MaskArgs a, int rows) {
+    touch_args<sizeof(MaskArgs) + sizeof(int)>();
     constexpr int ROWS = 8 / WAYS; // of a workgroup
     __shared__ float s_o[WAYS == 1 ? 1 : 8][D], s_ml[8][2];
     const int hw = (int)threadIdx.x >> 5, c = (int)threadIdx.x & 31;
@@ -930,8 +1048,9 @@ __global__ void __launch_bounds__(256) attn_masked_merge_kernel(const MaskArgs a
     const int per = a.q_tokens * a.group;
     const int sk = r / per;
     const int rr = r - sk * per;
-    const int kvh = sk % a.kv_heads, seq = sk / a.kv_heads;
-    const RowPos p{seq, rr / a.group, rr % a.group};
+    const int seq = sk / a.kv_heads, kvh = sk - seq * a.kv_heads;
+    const int tok = div24(rr, a.group);
+    const RowPos p{seq, tok, rr - tok * a.group};
     float m = -INFINITY, l = 0.f;
     f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
     auto add = [&](float ms, float ls, const f32x4& x) __attribute__((always_inline)) {

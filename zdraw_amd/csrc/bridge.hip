@@ -1965,7 +1965,7 @@ int set_job(MaskJob* j, const MaskLayout& y, int seqs, int kv_heads, int64_t row
     j->row_tiles = y.row_tiles;
     j->splits = y.splits;
     const int64_t wgs = (int64_t)seqs * kv_heads * y.row_tiles * y.splits;
-    if (wgs > 0x3fffffffLL) return unavailable("grid too large");
+    if (wgs >= (1 << 24)) return unavailable("grid too large");
     j->workgroups = (int32_t)wgs;
     return ZDRAW_HIP_OK;
 }
@@ -1995,7 +1995,8 @@ int plan_shared_jobs(const ZdrawHipSharedAttn* p, int cus, bool split_ok, MaskAr
     int rc;
     const bool both = p->prefix_tokens != 0 && p->capacity != 0;
     const bool full = rows >= 64 && (rows + 127) / 128 * groups >= cus / 2;
-    if (!both || !split_ok || full) {
+    const int64_t pooled = rows * p->requests;
+    if (!both || !split_ok || full || pooled >= (int64_t)kMaskMaxTokens) {
         a->jobs = 1;
         j0.spans = both ? 2 : 1;
         j0.kind[0] = both || p->prefix_tokens != 0 ? kRangePrefix : kRangeOwn;
@@ -2011,10 +2012,13 @@ int plan_shared_jobs(const ZdrawHipSharedAttn* p, int cus, bool split_ok, MaskAr
     j0.spans = j1.spans = 1;
     j0.kind[0] = kRangePrefix;
     j1.kind[0] = kRangeOwn;
-    const int64_t pooled = rows * p->requests;
-    if (pooled * p->kv_heads > 0x7fffffffLL / 2) return unavailable("too many rows");
-    const MaskLayout y0 = mask_layout(pooled, p->kv_heads, p->prefix_tokens, cus, true);
-    const MaskLayout y1 = mask_layout(rows, groups, p->capacity, cus, true);
+    MaskLayout y0 = mask_layout(pooled, p->kv_heads, p->prefix_tokens, cus, true);
+    MaskLayout y1 = mask_layout(rows, groups, p->capacity, cus, true);
+    // both are on the GPU at once: the workgroup slots are dealt out by the keys that each walks
+    const int64_t slots = 2 * (int64_t)cus, t0 = y0.row_tiles * (int64_t)p->kv_heads, t1 = y1.row_tiles * groups;
+    const double w0 = (double)t0 * p->prefix_tokens, w1 = (double)t1 * p->capacity;
+    y1.splits = (int)std::clamp<int64_t>((int64_t)((double)slots * w1 / (w0 + w1)) / t1, 1, y1.splits);
+    y0.splits = (int)std::clamp<int64_t>((slots - t1 * y1.splits) / t0, 1, y0.splits);
     if ((rc = set_job(&j0, y0, 1, (int)p->kv_heads, pooled, 1)) != ZDRAW_HIP_OK) return rc;
     if ((rc = set_job(&j1, y1, (int)p->requests, (int)p->kv_heads, rows, 0)) != ZDRAW_HIP_OK) return rc;
     j1.part_base = job_rows(j0);

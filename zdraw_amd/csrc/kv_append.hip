@@ -17,6 +17,7 @@ namespace app {
 
 template <typename TIn, typename TOut, int SLOTS>
 __global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {
+    touch_args<sizeof(AppendArgs)>();
     const int lane16 = (int)threadIdx.x & 15;
     const int d0 = lane16 * 8;
     const int slots = a.heads + 2 * a.kv_heads;

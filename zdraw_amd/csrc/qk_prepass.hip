@@ -31,26 +31,10 @@ constexpr int kPrepTokens = 4; // tokens (waves) per workgroup
 // still walk six groups, most of which repeat the last head (not measured).
 constexpr int64_t kThinTokens = 8192;
 
-// One word of every cache line of a kernel's BYTES of arguments, in one round trip. (Of the arguments themselves only: what
-// the runtime keeps behind them, the grid size among it, exists in the kernels that read it and in no others.)
-// The compiler loads arguments where they are first used: each line is a miss to memory (the host has just
-// written them) that the next waits for, at the head of every workgroup's chain, and the pre-pass has ten of them. Calls,
+// The arguments' ten cache lines are loaded at once (touch_args, attn_device.hpp). Calls,
 // us, without and with: 24 heads bf16, 768 tokens, five blocks 141.0 -> 138.9 (three pairs of runs, 1.3 to 2 %),
 // 4 x 1536 tokens, two blocks 310.7 -> 308.8. In the attention kernel and its merge (six lines), the
 // products (three) and the wide head (one) it shows in no call: 0.3 % and less.
-template <size_t BYTES>
-__device__ __forceinline__ void touch_args() {
-    constexpr int N = (int)((BYTES + 63) / 64);
-    static_assert(N >= 1 && N <= 12, "one operand per line below");
-    static_assert(BYTES % 4 == 0 && 64 * (N - 1) + 4 <= BYTES, "the last word lies within the arguments");
-    typedef const __attribute__((address_space(4))) unsigned* args_t;
-    const args_t p = (args_t)__builtin_amdgcn_kernarg_segment_ptr();
-    unsigned x[12];
-#pragma unroll
-    for (int i = 0; i < 12; i++) x[i] = p[16 * (i < N ? i : N - 1)];
-    asm volatile("" ::"s"(x[0]), "s"(x[1]), "s"(x[2]), "s"(x[3]), "s"(x[4]), "s"(x[5]), "s"(x[6]), "s"(x[7]), "s"(x[8]), "s"(x[9]), "s"(x[10]), "s"(x[11]));
-}
-
 template <typename TIn, int MODE, int G>
 __global__ void __launch_bounds__(kPrepTokens * 64) qk_prepass_kernel(const PrepPair pair) {
     touch_args<sizeof(PrepPair)>();
