@@ -649,14 +649,19 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
         const int whole_end = base.table ? 0 : lo + (hi - lo) / KB * KB; // up to here blocks lie in memory as they do in LDS
         const int n_down = blocks_down<MODE>(a, __builtin_amdgcn_readfirstlane(max(max(s_pos[i][0], s_pos[i][1]), max(s_pos[i][2], s_pos[i][3]))), lo, nb);
         auto first_key = [&](int b) __attribute__((always_inline)) { return lo + (b < n_down ? n_down - 1 - b : b) * KB; };
+        // (unbiased rows take blocks in their order: the address is carried along)
+        const char* k_next = base.k + (int64_t)(lo + 8 * wave) * sp.k_ts;
+        const char* v_next = base.v + (int64_t)(lo + 8 * wave) * sp.v_ts;
+        const int64_t k_step = (int64_t)KB * sp.k_ts, v_step = (int64_t)KB * sp.v_ts;
         const unsigned lds_w = lds0 + (unsigned)wave * 2048u;
         auto fetch_k = [&](int b) __attribute__((always_inline)) {
             const unsigned at = lds_w + (unsigned)(b & (kStages - 1)) * (unsigned)kBlock;
             const int j = first_key(b);
             if (j < whole_end) {
-                const char* const p = base.k + (int64_t)(j + 8 * wave) * sp.k_ts;
+                const char* const p = MODE == kPlain ? k_next : base.k + (int64_t)(j + 8 * wave) * sp.k_ts;
                 rows_to_lds(p, ko0, at);
                 rows_to_lds(p, ko1, at + 1024u);
+                if (MODE == kPlain) k_next += k_step;
             } else {
                 const int ln = lane_again();
                 load_rows<false>(sp, base, ln, j + 8 * wave, last, 2 * wave, at - (unsigned)wave * 2048u);
@@ -667,9 +672,10 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
             const unsigned at = lds_w + kV + (unsigned)(b & (kStages - 1)) * (unsigned)kBlock;
             const int j = first_key(b);
             if (j < whole_end) {
-                const char* const p = base.v + (int64_t)(j + 8 * wave) * sp.v_ts;
+                const char* const p = MODE == kPlain ? v_next : base.v + (int64_t)(j + 8 * wave) * sp.v_ts;
                 rows_to_lds(p, vo0, at);
                 rows_to_lds(p, vo1, at + 1024u);
+                if (MODE == kPlain) v_next += v_step;
             } else {
                 const int ln = lane_again();
                 load_rows<true>(sp, base, ln, j + 8 * wave, last, 2 * wave, at - (unsigned)wave * 2048u);
