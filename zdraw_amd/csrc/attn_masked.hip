@@ -75,6 +75,13 @@ struct Range {
     bool live; // false: the row belongs to no sequence and is not written
 };
 
+// The lane's number formed anew, so that what is made from it in a seldom taken branch holds no register outside of it.
+__device__ __forceinline__ int lane_again() {
+    int x;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(x));
+    return x;
+}
+
 __device__ __forceinline__ RowPos row_pos(const MaskArgs& a, const MaskJob& job, int seq, int r) {
     RowPos p;
     const int t = div24(r, a.group);
@@ -98,13 +105,32 @@ __device__ __forceinline__ Range row_range(const MaskArgs& a, int kind, const Ke
         if (a.q_starts) {
             const unsigned* const qb = a.q_starts + (int64_t)p.seq * (a.documents + 1);
             const unsigned* const kb = a.k_starts + (int64_t)p.seq * (a.documents + 1);
-            int d = 0, top = a.documents; // the last border at or below the row
-            while (top - d > 1) {
-                const int mid = (d + top) >> 1;
-                if (qb[mid] <= (unsigned)p.tok) d = mid;
-                else top = mid;
+            int d = 0; // the last border at or below the row
+            unsigned s0, s1;
+            if (a.documents < 64) {
+                // a border a lane, one load; the rows of a wave ascend by less than 32 and differ by few documents
+                const int lane = lane_again();
+                const unsigned mine = qb[min(lane, a.documents)];
+                const unsigned low = (unsigned)__builtin_amdgcn_readfirstlane(p.tok);
+                const unsigned long long below = __builtin_amdgcn_ballot_w64(lane < a.documents && mine <= low);
+                d = max(63 - __builtin_clzll(below | 1ull), 0);
+                for (int x = __builtin_amdgcn_readfirstlane(d) + 1; x < a.documents; x++) {
+                    const unsigned border = (unsigned)__builtin_amdgcn_readlane((int)mine, x);
+                    if (__builtin_amdgcn_ballot_w64(border <= (unsigned)p.tok) == 0) break;
+                    d = border <= (unsigned)p.tok ? x : d;
+                }
+                s0 = qb[d];
+                s1 = qb[d + 1];
+            } else {
+                int top = a.documents;
+                while (top - d > 1) {
+                    const int mid = (d + top) >> 1;
+                    if (qb[mid] <= (unsigned)p.tok) d = mid;
+                    else top = mid;
+                }
+                s0 = qb[d];
+                s1 = qb[d + 1];
             }
-            const unsigned s0 = qb[d], s1 = qb[d + 1];
             r.live = s0 <= (unsigned)p.tok && (unsigned)p.tok < s1;
             qs = r.live ? (int)s0 : 0;
             qe = (int)min(s1, (unsigned)a.q_tokens);
@@ -173,16 +199,18 @@ __device__ __forceinline__ WaveRange wave_range(const MaskArgs& a, const MaskJob
     return w;
 }
 
-__device__ __forceinline__ int wave_min(int x) {
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) x = min(x, __shfl_xor(x, o));
-    return __builtin_amdgcn_readfirstlane(x);
+// Over the 32 rows of a wave (both halves hold them): four exchanges inside 16 lanes, and two lanes read.
+template <bool MAX>
+__device__ __forceinline__ int rows_extreme(int x) {
+    auto take = [](int p, int q) __attribute__((always_inline)) { return MAX ? max(p, q) : min(p, q); };
+    x = take(x, __builtin_amdgcn_update_dpp(x, x, 0xB1, 0xF, 0xF, true));  // quad_perm [1,0,3,2]
+    x = take(x, __builtin_amdgcn_update_dpp(x, x, 0x4E, 0xF, 0xF, true));  // quad_perm [2,3,0,1]
+    x = take(x, __builtin_amdgcn_update_dpp(x, x, 0x141, 0xF, 0xF, true)); // row_half_mirror
+    x = take(x, __builtin_amdgcn_update_dpp(x, x, 0x140, 0xF, 0xF, true)); // row_mirror
+    return take(__builtin_amdgcn_readlane(x, 0), __builtin_amdgcn_readlane(x, 16));
 }
-__device__ __forceinline__ int wave_max(int x) {
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) x = max(x, __shfl_xor(x, o));
-    return __builtin_amdgcn_readfirstlane(x);
-}
+__device__ __forceinline__ int wave_min(int x) { return rows_extreme<false>(x); }
+__device__ __forceinline__ int wave_max(int x) { return rows_extreme<true>(x); }
 
 // Address of key row j of a sequence and head; what is passed is uniform over the wave.
 struct SpanBase {
@@ -217,13 +245,6 @@ __device__ __forceinline__ void row_at(const KeySpan& sp, const SpanBase& b, int
     }
 }
 
-// The lane's number formed anew, so that what is made from it in a seldom taken branch holds no register outside of it.
-__device__ __forceinline__ int lane_again() {
-    int x;
-    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(x));
-    return x;
-}
-
 // A load takes four rows: lane i the 16-byte chunk of row i / 16 that the swizzle places at chunk i % 16 of LDS row 4 n + i / 16.
 __device__ __forceinline__ unsigned k_chunk(int lane, int n) { return (((unsigned)lane & 15u) ^ ((4u * (unsigned)n + ((unsigned)lane >> 4)) & 15u)) * 16u; }
 __device__ __forceinline__ unsigned v_chunk(int lane) { return (((unsigned)lane & 15u) ^ (((unsigned)lane >> 4) << 2)) * 16u; }
@@ -244,12 +265,23 @@ __device__ __forceinline__ void load_rows(const KeySpan& sp, const SpanBase& b, 
 template <bool V>
 __device__ __forceinline__ void load_block(const KeySpan& sp, const SpanBase& b, int lane, const unsigned (&off)[4], int j, int last, unsigned lds) {
     const unsigned ts = (unsigned)(V ? sp.v_ts : sp.k_ts);
-    if (!sp.table && j + KB - 1 <= last) {
-        const char* p = V ? b.v + (int64_t)j * ts : b.k + (int64_t)j * ts;
+    if ((!sp.table || sp.page_mask >= 15) && j + KB - 1 <= last) { // (blocks of a paged span start at multiples of 32)
+        const char *kp[2], *vp[2];
+        row_at(sp, b, j, kp[0], vp[0]);
+        if (sp.table && sp.page_mask == 15) {
+            row_at(sp, b, j + 16, kp[1], vp[1]);
+        } else {
+            kp[1] = kp[0] + 16 * (int64_t)ts;
+            vp[1] = vp[0] + 16 * (int64_t)ts;
+        }
 #pragma unroll
-        for (int n = 0; n < 8; n++) {
-            rows_to_lds(p, off[V ? 0 : n & 3], lds + (unsigned)n * 1024u);
-            p += 4 * (int64_t)ts;
+        for (int g = 0; g < 2; g++) {
+            const char* p = V ? vp[g] : kp[g];
+#pragma unroll
+            for (int n = 4 * g; n < 4 * g + 4; n++) {
+                rows_to_lds(p, off[V ? 0 : n & 3], lds + (unsigned)n * 1024u);
+                p += 4 * (int64_t)ts;
+            }
         }
         return;
     }
@@ -477,14 +509,31 @@ struct Item {
     int sk, seq, kvh, tile, split;
 };
 __device__ __forceinline__ Item item_of(const MaskArgs& a, const MaskJob& job, int id) {
-    // consecutive items on one XCD, whose L2 then serves the tiles that walk the same keys
-    const int xcd = id & 7, idx = id >> 3, per = job.workgroups >> 3, rem = job.workgroups & 7;
-    const int item = idx + xcd * per + min(xcd, rem);
+    // A head's items go to one XCD, whose L2 then serves the tiles that walk the same keys; heads are dealt out to the XCDs in
+    // turn (sequences of different length come in runs of heads), the last few of them, fewer than XCDs, item by item.
+    const int per_sk = job.row_tiles * job.splits, sks = job.seqs * a.kv_heads, turns = sks >> 3;
+    const int xcd = id & 7, idx = id >> 3;
     Item it;
-    const int rest = div24(item, job.row_tiles);
-    it.tile = job.row_tiles - 1 - (item - rest * job.row_tiles); // the last rows see the most keys: first
-    it.sk = div24(rest, job.splits);
-    it.split = rest - it.sk * job.splits;
+    int within;
+    if (idx < turns * per_sk) {
+        int turn;
+        if (job.interleave) { // an XCD's heads side by side: their keys fit its L2, and the tiles that see most come first
+            within = div24(idx, turns);
+            turn = idx - within * turns;
+        } else {
+            turn = div24(idx, per_sk);
+            within = idx - turn * per_sk;
+        }
+        it.sk = turn * 8 + xcd;
+    } else {
+        const int left = (sks - 8 * turns) * per_sk, per = left >> 3, rem = left & 7;
+        const int x = idx - turns * per_sk + xcd * per + min(xcd, rem);
+        it.sk = div24(x, per_sk);
+        within = x - it.sk * per_sk;
+        it.sk += 8 * turns;
+    }
+    it.split = div24(within, job.row_tiles);
+    it.tile = job.row_tiles - 1 - (within - it.split * job.row_tiles); // the last rows see the most keys: first
     it.seq = div24(it.sk, a.kv_heads);
     it.kvh = it.sk - it.seq * a.kv_heads;
     it.tile = __builtin_amdgcn_readfirstlane(it.tile);
@@ -1103,7 +1152,13 @@ __global__ void __launch_bounds__(256) attn_masked_merge_kernel(const MaskArgs a
 #pragma unroll
         for (int w = 0; w < WAYS; w++) add(s_ml[hw + w][0], s_ml[hw + w][1], *reinterpret_cast<const f32x4*>(&s_o[hw + w][4 * c]));
     }
-    if (!mine || !row_range(a, a.job[0].kind[0], a.job[0].span[0], p).live) return;
+    bool live = mine; // as row_range has it, where borders ascend
+    if (a.q_starts) {
+        const unsigned* const qb = a.q_starts + (int64_t)p.seq * (a.documents + 1);
+        live = live && qb[0] <= (unsigned)p.tok && (unsigned)p.tok < qb[a.documents];
+    }
+    if (a.q_lens) live = live && (unsigned)p.tok < a.q_lens[p.seq];
+    if (!live) return;
     const float inv = l == 0.f ? 0.f : 1.0f / l;
     char* const out = a.o + (int64_t)seq * a.o_ss + (int64_t)p.tok * a.o_ts + (int64_t)(kvh * a.group + p.g) * a.o_hs;
     *reinterpret_cast<u32x2*>(out + 8 * c) = u32x2{round2<F16>(o[0] * inv, o[1] * inv), round2<F16>(o[2] * inv, o[3] * inv)};
