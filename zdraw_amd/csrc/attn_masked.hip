@@ -148,8 +148,8 @@ __device__ __forceinline__ Range row_range(const MaskArgs& a, int kind, const Ke
         r.pos = ks + at;
     } else {
         // (of the prefix, what a request holds itself counts for the bias alone)
-        const int n = a.lens && (kind != kRangePrefix || a.slopes) ? (int)min(a.lens[p.seq], (unsigned)a.own_keys) : 0;
-        const int ql = a.q_lens ? (int)min(a.q_lens[p.seq], (unsigned)a.q_tokens) : a.q_tokens;
+        const int n = a.lens && (kind != kRangePrefix || a.slopes) ? (int)min(((const_u32_t)a.lens)[p.seq], (unsigned)a.own_keys) : 0;
+        const int ql = a.q_lens ? (int)min(((const_u32_t)a.q_lens)[p.seq], (unsigned)a.q_tokens) : a.q_tokens;
         r.live = p.tok < ql;
         const int at = p.tok + n - ql;
         if (kind == kRangePrefix) {
@@ -1024,14 +1024,17 @@ __global__ void __launch_bounds__(256, 2) attn_keys_kernel(const MaskArgs a, con
         s_ml[wave][l32][1] = st.l;
     }
     unsigned char* const mine = smem + wave * (2 * kBlock); // 32 x 512 bytes, 16-byte chunks swizzled by row
+    if (here) {
 #pragma unroll
-    for (int b = 0; b < 4; b++)
+        for (int b = 0; b < 4; b++)
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            *reinterpret_cast<f32x4*>(mine + l32 * (2 * kRow) + (((8 * b + 2 * i + h) ^ l32) * 16)) =
-                f32x4{st.o[b][4 * i], st.o[b][4 * i + 1], st.o[b][4 * i + 2], st.o[b][4 * i + 3]};
+            for (int i = 0; i < 4; i++)
+                *reinterpret_cast<f32x4*>(mine + l32 * (2 * kRow) + (((8 * b + 2 * i + h) ^ l32) * 16)) =
+                    f32x4{st.o[b][4 * i], st.o[b][4 * i + 1], st.o[b][4 * i + 2], st.o[b][4 * i + 3]};
+    }
     __syncthreads();
     const int rr = tid >> 3, c8 = tid & 7; // eight threads a row, 16 dims each
+    const bool mine_live = ((unsigned)__builtin_amdgcn_ballot_w64(here) >> rr) & 1u;
     float m = -INFINITY;
 #pragma unroll
     for (int w = 0; w < 4; w++) m = fmaxf(m, s_ml[w][rr][0]);
@@ -1042,7 +1045,7 @@ __global__ void __launch_bounds__(256, 2) attn_keys_kernel(const MaskArgs a, con
 #pragma unroll
     for (int w = 0; w < 4; w++) {
         const float mw = s_ml[w][rr][0], lw = s_ml[w][rr][1];
-        if (lw == 0.f) continue; // (a share without keys)
+        if (!mine_live || lw == 0.f) continue; // (a share without keys)
         const float f = __builtin_amdgcn_exp2f(mw - m);
         l += f * lw;
 #pragma unroll
@@ -1059,8 +1062,6 @@ __global__ void __launch_bounds__(256, 2) attn_keys_kernel(const MaskArgs a, con
         for (int j = 0; j < 4; j++) z = __builtin_fmaf(o[i][j], 0.0f, z);
 #pragma unroll
     for (int x = 1; x < 8; x <<= 1) z += __shfl_xor(z, x);
-    const unsigned alive = (unsigned)__builtin_amdgcn_ballot_w64(here);
-    const bool mine_live = (alive >> rr) & 1u;
     const bool again = mine_live && !(z == 0.f);
     if (again && c8 == 0) atomicOr(&s_bad, 1u << rr);
     if (mine_live && !again) {
