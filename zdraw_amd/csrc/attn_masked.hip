@@ -509,31 +509,33 @@ struct Item {
     int sk, seq, kvh, tile, split;
 };
 __device__ __forceinline__ Item item_of(const MaskArgs& a, const MaskJob& job, int id) {
-    // A head's items go to one XCD, whose L2 then serves the tiles that walk the same keys; heads are dealt out to the XCDs in
-    // turn (sequences of different length come in runs of heads), the last few of them, fewer than XCDs, item by item.
-    const int per_sk = job.row_tiles * job.splits, sks = job.seqs * a.kv_heads, turns = sks >> 3;
-    const int xcd = id & 7, idx = id >> 3;
+    const int sks = job.seqs * a.kv_heads;
     Item it;
-    int within;
-    if (idx < turns * per_sk) {
-        int turn;
-        if (job.interleave) { // an XCD's heads side by side: their keys fit its L2, and the tiles that see most come first
-            within = div24(idx, turns);
-            turn = idx - within * turns;
-        } else {
-            turn = div24(idx, per_sk);
-            within = idx - turn * per_sk;
-        }
-        it.sk = turn * 8 + xcd;
+    if (!job.by_keys) {
+        // Tile by tile over all heads, the tiles that see the most keys first: the GPU's last workgroups are its shortest. The
+        // heads' turn is also the XCDs' where their number is a multiple of 8; tiles that walk the same keys start together
+        // and share them in the L2. (Head by head on an XCD, 24 heads of 4096 causal tokens: 126 us, so 109.)
+        const int w = div24(id, sks);
+        it.sk = id - w * sks;
+        it.split = div24(w, job.row_tiles);
+        it.tile = job.row_tiles - 1 - (w - it.split * job.row_tiles);
     } else {
-        const int left = (sks - 8 * turns) * per_sk, per = left >> 3, rem = left & 7;
-        const int x = idx - turns * per_sk + xcd * per + min(xcd, rem);
-        it.sk = div24(x, per_sk);
-        within = x - it.sk * per_sk;
-        it.sk += 8 * turns;
+        // The tiles that walk the same share of a head's keys follow each other on one XCD.
+        const int groups = sks * job.splits, turns = groups >> 3, idx = id >> 3;
+        int group;
+        if (idx < turns * job.row_tiles) {
+            const int turn = div24(idx, job.row_tiles);
+            it.tile = idx - turn * job.row_tiles;
+            group = turn * 8 + (id & 7);
+        } else { // the last few shares, fewer than XCDs, tile by tile
+            const int x = id - 8 * turns * job.row_tiles, g = div24(x, job.row_tiles);
+            it.tile = x - g * job.row_tiles;
+            group = 8 * turns + g;
+        }
+        it.tile = job.row_tiles - 1 - it.tile;
+        it.split = div24(group, sks);
+        it.sk = group - it.split * sks;
     }
-    it.split = div24(within, job.row_tiles);
-    it.tile = job.row_tiles - 1 - (within - it.split * job.row_tiles); // the last rows see the most keys: first
     it.seq = div24(it.sk, a.kv_heads);
     it.kvh = it.sk - it.seq * a.kv_heads;
     it.tile = __builtin_amdgcn_readfirstlane(it.tile);

@@ -1957,7 +1957,7 @@ MaskLayout mask_layout(int64_t rows, int64_t groups, int64_t keys, int cus, bool
 
 int64_t job_rows(const MaskJob& j) { return (int64_t)j.workgroups * (j.by_keys ? kMaskRowsByKeys : kMaskRowsByWave); }
 
-int set_job(MaskJob* j, const MaskLayout& y, int seqs, int kv_heads, int64_t rows, int64_t keys, int pooled) {
+int set_job(MaskJob* j, const MaskLayout& y, int seqs, int kv_heads, int64_t rows, int pooled) {
     j->by_keys = y.by_keys;
     j->seqs = seqs;
     j->pooled = pooled;
@@ -1967,8 +1967,6 @@ int set_job(MaskJob* j, const MaskLayout& y, int seqs, int kv_heads, int64_t row
     const int64_t wgs = (int64_t)seqs * kv_heads * y.row_tiles * y.splits;
     if (wgs >= (1 << 24)) return unavailable("grid too large");
     j->workgroups = (int32_t)wgs;
-    // (an XCD's L2 is 4 MB; a key and its value are 512 bytes)
-    j->interleave = keys * 2 * kHeadDim * 2 * ((seqs * (int64_t)kv_heads + 7) / 8) <= (3 << 20);
     return ZDRAW_HIP_OK;
 }
 
@@ -1980,7 +1978,7 @@ int plan_masked_jobs(const ZdrawHipMaskedAttn* p, int cus, bool split_ok, MaskAr
     j.spans = 1;
     j.kind[0] = kRangeDocs;
     const MaskLayout y = mask_layout(rows, (int64_t)p->batch * p->kv_heads, p->k_tokens, cus, split_ok);
-    const int rc = set_job(&j, y, (int)p->batch, (int)p->kv_heads, rows, p->k_tokens, 0);
+    const int rc = set_job(&j, y, (int)p->batch, (int)p->kv_heads, rows, 0);
     if (rc != ZDRAW_HIP_OK) return rc;
     a->direct = j.splits == 1;
     *part_rows = a->direct ? 0 : (size_t)job_rows(j);
@@ -2004,7 +2002,7 @@ int plan_shared_jobs(const ZdrawHipSharedAttn* p, int cus, bool split_ok, MaskAr
         j0.kind[0] = both || p->prefix_tokens != 0 ? kRangePrefix : kRangeOwn;
         j0.kind[1] = kRangeOwn;
         MaskLayout y = mask_layout(rows, groups, (int64_t)p->prefix_tokens + p->capacity, cus, split_ok && !both);
-        if ((rc = set_job(&j0, y, (int)p->requests, (int)p->kv_heads, rows, (int64_t)p->prefix_tokens + p->capacity, 0)) != ZDRAW_HIP_OK) return rc;
+        if ((rc = set_job(&j0, y, (int)p->requests, (int)p->kv_heads, rows, 0)) != ZDRAW_HIP_OK) return rc;
         a->direct = j0.splits == 1;
         *part_rows = a->direct ? 0 : (size_t)job_rows(j0);
         return ZDRAW_HIP_OK;
@@ -2021,8 +2019,8 @@ int plan_shared_jobs(const ZdrawHipSharedAttn* p, int cus, bool split_ok, MaskAr
     const double w0 = (double)t0 * p->prefix_tokens, w1 = (double)t1 * p->capacity;
     y1.splits = (int)std::clamp<int64_t>((int64_t)((double)slots * w1 / (w0 + w1)) / t1, 1, y1.splits);
     y0.splits = (int)std::clamp<int64_t>((slots - t1 * y1.splits) / t0, 1, y0.splits);
-    if ((rc = set_job(&j0, y0, 1, (int)p->kv_heads, pooled, p->prefix_tokens, 1)) != ZDRAW_HIP_OK) return rc;
-    if ((rc = set_job(&j1, y1, (int)p->requests, (int)p->kv_heads, rows, p->capacity, 0)) != ZDRAW_HIP_OK) return rc;
+    if ((rc = set_job(&j0, y0, 1, (int)p->kv_heads, pooled, 1)) != ZDRAW_HIP_OK) return rc;
+    if ((rc = set_job(&j1, y1, (int)p->requests, (int)p->kv_heads, rows, 0)) != ZDRAW_HIP_OK) return rc;
     j1.part_base = job_rows(j0);
     *part_rows = (size_t)(job_rows(j0) + job_rows(j1));
     return ZDRAW_HIP_OK;

@@ -36,7 +36,6 @@ struct MaskJob {
     int32_t rows;      // per sequence
     int32_t row_tiles, splits;
     int32_t workgroups; // seqs * kv_heads * row_tiles * splits
-    int32_t interleave; // 1: tile by tile over an XCD's heads, 0: head by head
     int64_t part_base; // first row of this job's parts in part_o / part_ml
 };
 
