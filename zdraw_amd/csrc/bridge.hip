@@ -1977,7 +1977,13 @@ int plan_masked_jobs(const ZdrawHipMaskedAttn* p, int cus, bool split_ok, MaskAr
     MaskJob& j = a->job[0];
     j.spans = 1;
     j.kind[0] = kRangeDocs;
-    const MaskLayout y = mask_layout(rows, (int64_t)p->batch * p->kv_heads, p->k_tokens, cus, split_ok);
+    MaskLayout y = mask_layout(rows, (int64_t)p->batch * p->kv_heads, p->k_tokens, cus, split_ok);
+    // Tiles that keep to their documents: where a document fills one on average (shorter ones share tiles), and a lane of a
+    // wave holds each.
+    if (!y.by_keys && y.splits == 1 && p->documents > 0 && p->documents < 64 && rows / p->documents >= kMaskRowsByWave) {
+        y.row_tiles += (int)p->documents;
+        j.by_document = 1;
+    }
     const int rc = set_job(&j, y, (int)p->batch, (int)p->kv_heads, rows, 0);
     if (rc != ZDRAW_HIP_OK) return rc;
     a->direct = j.splits == 1;

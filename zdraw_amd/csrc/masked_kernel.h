@@ -35,6 +35,7 @@ struct MaskJob {
     int32_t pooled;    // 1: the rows of all sequences are one row space (seqs == 1)
     int32_t rows;      // per sequence
     int32_t row_tiles, splits;
+    int32_t by_document; // 1: tiles keep to the documents, row_tiles is the most that there can be
     int32_t workgroups; // seqs * kv_heads * row_tiles * splits
     int64_t part_base; // first row of this job's parts in part_o / part_ml
 };
