@@ -51,6 +51,11 @@ __device__ __forceinline__ void pin(T& v) {
     asm volatile("" : "+v"(v));
 }
 
+// The same with an address a lane.
+__device__ __forceinline__ void row_to_lds(const char* at, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(at) : "memory", "m0");
+}
+
 template <int N>
 __device__ __forceinline__ void wait_loads() {
     asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
@@ -96,108 +101,119 @@ __device__ __forceinline__ RowPos row_pos(const MaskArgs& a, const MaskJob& job,
     return p;
 }
 
-__device__ __forceinline__ Range row_range(const MaskArgs& a, int kind, const KeySpan& sp, const RowPos& p) {
-    Range r;
-    r.lo = 0;
-    r.live = true;
-    if (kind == kRangeDocs) {
-        int qs = 0, qe = a.q_tokens, ks = 0, ke = sp.keys, pre = 0, doc = 0;
-        if (a.q_starts) {
-            const unsigned* const qb = a.q_starts + (int64_t)p.seq * (a.documents + 1);
-            const unsigned* const kb = a.k_starts + (int64_t)p.seq * (a.documents + 1);
-            int d = 0; // the last border at or below the row
-            unsigned s0, s1;
-            if (a.documents < 64) {
-                // a border a lane, one load; the rows of a wave ascend by less than 32 and differ by few documents
-                const int lane = lane_again();
-                const unsigned mine = qb[min(lane, a.documents)];
-                const unsigned low = (unsigned)__builtin_amdgcn_readfirstlane(p.tok);
-                const unsigned long long below = __builtin_amdgcn_ballot_w64(lane < a.documents && mine <= low);
-                d = max(63 - __builtin_clzll(below | 1ull), 0);
-                for (int x = __builtin_amdgcn_readfirstlane(d) + 1; x < a.documents; x++) {
-                    const unsigned border = (unsigned)__builtin_amdgcn_readlane((int)mine, x);
-                    if (__builtin_amdgcn_ballot_w64(border <= (unsigned)p.tok) == 0) break;
-                    d = border <= (unsigned)p.tok ? x : d;
-                }
-                s0 = qb[d];
-                s1 = qb[d + 1];
-            } else {
-                int top = a.documents;
-                while (top - d > 1) {
-                    const int mid = (d + top) >> 1;
-                    if (qb[mid] <= (unsigned)p.tok) d = mid;
-                    else top = mid;
-                }
-                s0 = qb[d];
-                s1 = qb[d + 1];
-            }
-            r.live = s0 <= (unsigned)p.tok && (unsigned)p.tok < s1;
-            qs = r.live ? (int)s0 : 0;
-            qe = (int)min(s1, (unsigned)a.q_tokens);
-            ks = (int)min(kb[d], (unsigned)sp.keys);
-            ke = max((int)min(kb[d + 1], (unsigned)sp.keys), ks);
-            doc = d;
+// A document: its query rows [qs, qe), keys [ks, ke), and how many of those all of its rows see.
+struct Doc {
+    int qs, qe, ks, ke, pre;
+};
+// (borders held to the sequence)
+__device__ __forceinline__ Doc doc_of_borders(const MaskArgs& a, unsigned q0, unsigned q1, unsigned k0, unsigned k1, unsigned pre, int keys) {
+    Doc d;
+    d.qe = (int)min(q1, (unsigned)a.q_tokens);
+    d.qs = min((int)min(q0, (unsigned)a.q_tokens), d.qe);
+    d.ks = (int)min(k0, (unsigned)keys);
+    d.ke = max((int)min(k1, (unsigned)keys), d.ks);
+    d.pre = (int)min(pre, (unsigned)(d.ke - d.ks));
+    return d;
+}
+// The d-th document of a sequence; d may differ from lane to lane.
+__device__ __forceinline__ Doc doc_at(const MaskArgs& a, int seq, int d, int keys) {
+    const const_u32_t qb = (const_u32_t)a.q_starts + (int64_t)seq * (a.documents + 1), kb = (const_u32_t)a.k_starts + (int64_t)seq * (a.documents + 1);
+    return doc_of_borders(a, qb[d], qb[d + 1], kb[d], kb[d + 1], a.prefix ? ((const_u32_t)a.prefix)[(int64_t)seq * a.documents + d] : 0u, keys);
+}
+// The document that a row lies in. `ascending`: the lanes' rows ascend by less than 32 inside one sequence; then a lane
+// holds each of up to 63 documents' borders, all loaded in one round trip, and few are looked at.
+__device__ __forceinline__ Doc doc_of_row(const MaskArgs& a, int seq, int tok, int keys, bool ascending) {
+    if (!a.q_starts) return doc_of_borders(a, 0u, (unsigned)a.q_tokens, 0u, (unsigned)keys, a.prefix ? ((const_u32_t)a.prefix)[seq] : 0u, keys);
+    const unsigned* const qb = a.q_starts + (int64_t)seq * (a.documents + 1);
+    int d = 0; // the last border at or below the row
+    if (ascending && a.documents < 64) {
+        const int lane = lane_again(), mine = min(lane, a.documents);
+        const unsigned q = qb[mine], k = a.k_starts[(int64_t)seq * (a.documents + 1) + mine];
+        const unsigned pre = a.prefix ? a.prefix[(int64_t)seq * a.documents + min(lane, a.documents - 1)] : 0u;
+        const unsigned long long below = __builtin_amdgcn_ballot_w64(lane < a.documents && q <= (unsigned)__builtin_amdgcn_readfirstlane(tok));
+        d = 63 - __builtin_clzll(below | 1ull);
+        for (int x = __builtin_amdgcn_readfirstlane(d) + 1; x < a.documents; x++) {
+            const unsigned border = (unsigned)__builtin_amdgcn_readlane((int)q, x);
+            if (__builtin_amdgcn_ballot_w64(border <= (unsigned)tok) == 0) break;
+            d = border <= (unsigned)tok ? x : d;
         }
-        if (a.prefix) pre = (int)min(a.prefix[(int64_t)p.seq * max(a.documents, 1) + doc], (unsigned)(ke - ks));
-        const int nk = ke - ks;
-        const int at = p.tok - qs + nk - (qe - qs); // the last query stands on the last key
-        int n = a.causal ? max(min(at + 1, nk), pre) : nk;
-        n = r.live ? max(n, 0) : 0;
-        r.lo = ks;
-        r.hi = ks + n;
-        r.pos = ks + at;
-    } else {
-        // (of the prefix, what a request holds itself counts for the bias alone)
-        const int n = a.lens && (kind != kRangePrefix || a.slopes) ? (int)min(((const_u32_t)a.lens)[p.seq], (unsigned)a.own_keys) : 0;
-        const int ql = a.q_lens ? (int)min(((const_u32_t)a.q_lens)[p.seq], (unsigned)a.q_tokens) : a.q_tokens;
-        r.live = p.tok < ql;
-        const int at = p.tok + n - ql;
-        if (kind == kRangePrefix) {
-            r.hi = sp.keys;
-            r.pos = sp.keys + at;
-        } else {
-            r.hi = a.causal ? max(min(at + 1, n), 0) : n;
-            r.pos = at;
-        }
-        if (!r.live) r.hi = 0;
+        return doc_of_borders(a, (unsigned)__shfl((int)q, d), (unsigned)__shfl((int)q, d + 1), (unsigned)__shfl((int)k, d), (unsigned)__shfl((int)k, d + 1),
+                              (unsigned)__shfl((int)pre, d), keys);
     }
+    int top = a.documents;
+    while (top - d > 1) {
+        const int mid = (d + top) >> 1;
+        if (qb[mid] <= (unsigned)tok) d = mid;
+        else top = mid;
+    }
+    return doc_at(a, seq, d, keys);
+}
+
+__device__ __forceinline__ Range range_in(const MaskArgs& a, const Doc& d, int tok) {
+    Range r;
+    r.live = d.qs <= tok && tok < d.qe;
+    const int nk = d.ke - d.ks;
+    const int at = tok - d.qs + nk - (d.qe - d.qs); // the last query stands on the last key
+    const int n = a.causal ? max(min(at + 1, nk), d.pre) : nk;
+    r.lo = d.ks;
+    r.hi = d.ks + (r.live ? max(n, 0) : 0);
+    r.pos = d.ks + at;
     return r;
 }
 
-// What the rows of a wave see together: from the first to the last key of any row, and what every row sees. `first_row`,
-// `last_row`: of the wave's rows, held to the sequence. Inside a document, or without any, the ranges of its rows only grow.
+// The keys of a row that sees the shared prefix, or its request's own.
+__device__ __forceinline__ Range request_range(const MaskArgs& a, int kind, const KeySpan& sp, const RowPos& p) {
+    Range r;
+    r.lo = 0;
+    // (of the prefix, what a request holds itself counts for the bias alone)
+    const int n = a.lens && (kind != kRangePrefix || a.slopes) ? (int)min(((const_u32_t)a.lens)[p.seq], (unsigned)a.own_keys) : 0;
+    const int ql = a.q_lens ? (int)min(((const_u32_t)a.q_lens)[p.seq], (unsigned)a.q_tokens) : a.q_tokens;
+    r.live = p.tok < ql;
+    const int at = p.tok + n - ql;
+    if (kind == kRangePrefix) {
+        r.hi = sp.keys;
+        r.pos = sp.keys + at;
+    } else {
+        r.hi = a.causal ? max(min(at + 1, n), 0) : n;
+        r.pos = at;
+    }
+    if (!r.live) r.hi = 0;
+    return r;
+}
+
+// What the rows of a wave see together: from the first to the last key of any row, and what every row sees.
 struct WaveRange {
     int lo, hi, all_lo, all_hi;
     int pos_lo, pos_hi; // where the first and the last row stand
 };
 __device__ __forceinline__ int wave_min(int x);
 __device__ __forceinline__ int wave_max(int x);
-__device__ __forceinline__ WaveRange wave_range(const MaskArgs& a, const MaskJob& job, int kind, const KeySpan& sp, int seq, int first_row, int last_row, const Range& r) {
-    WaveRange w;
-    if ((kind == kRangeDocs && a.q_starts && !job.by_document) || (job.pooled && a.q_lens)) {
-        const bool some = r.hi > r.lo;
-        w.lo = wave_min(some ? r.lo : 0x7fffffff);
-        w.hi = wave_max(some ? r.hi : 0);
-        w.all_lo = wave_max(r.lo);
-        w.all_hi = wave_min(r.hi);
-        w.pos_lo = wave_min(r.pos);
-        w.pos_hi = wave_max(r.pos);
-        return w;
+__device__ __forceinline__ WaveRange wave_range_of(const Range& r) {
+    const bool some = r.hi > r.lo;
+    return WaveRange{wave_min(some ? r.lo : 0x7fffffff), wave_max(some ? r.hi : 0), wave_max(r.lo), wave_min(r.hi), wave_min(r.pos), wave_max(r.pos)};
+}
+// The same where ranges only grow from the first row's to the last one's: inside a document, a request or the prefix. (Rows
+// past their request's, behind the last live one, see nothing.)
+__device__ __forceinline__ WaveRange wave_range_of(const Range& first, const Range& last, const Range& r) {
+    const int hi = last.live ? last.hi : wave_max(r.hi);
+    return WaveRange{first.lo, hi, first.lo, last.live ? first.hi : 0, first.pos, last.pos};
+}
+// Rows [first_row, last_row] of a wave, r its lanes' own (doc: of its rows, where it is one).
+__device__ __forceinline__ Range lane_range(const MaskArgs& a, const MaskJob& job, int kind, const KeySpan& sp, const RowPos& rp, const Doc& doc) {
+    if (kind != kRangeDocs) return request_range(a, kind, sp, rp);
+    if (job.by_document || !a.q_starts) return range_in(a, doc, rp.tok);
+    return range_in(a, doc_of_row(a, rp.seq, rp.tok, sp.keys, true), rp.tok);
+}
+__device__ __forceinline__ WaveRange wave_range(const MaskArgs& a, const MaskJob& job, int kind, const KeySpan& sp, int seq, int first_row, int last_row, const Range& r,
+                                                const Doc& doc) {
+    if (kind == kRangeDocs && a.q_starts && !job.by_document) return wave_range_of(r);
+    if (job.pooled) {
+        if (a.q_lens || a.slopes) return wave_range_of(r);
+        return WaveRange{0, sp.keys, 0, sp.keys, 0, 0};
     }
-    if (job.pooled) { // (the prefix)
-        w.lo = w.all_lo = 0;
-        w.hi = w.all_hi = sp.keys;
-        w.pos_lo = a.slopes ? wave_min(r.pos) : 0;
-        w.pos_hi = a.slopes ? wave_max(r.pos) : 0;
-        return w;
-    }
-    const Range lo = row_range(a, kind, sp, RowPos{seq, div24(first_row, a.group), 0}), hi = row_range(a, kind, sp, RowPos{seq, div24(last_row, a.group), 0});
-    w.lo = w.all_lo = lo.lo; // (the first key of the document)
-    w.all_hi = hi.live ? lo.hi : 0;
-    w.hi = hi.live ? hi.hi : wave_max(r.hi);
-    w.pos_lo = lo.pos;
-    w.pos_hi = hi.pos;
-    return w;
+    const int t0 = div24(first_row, a.group), t1 = div24(last_row, a.group);
+    if (kind == kRangeDocs) return wave_range_of(range_in(a, doc, t0), range_in(a, doc, t1), r);
+    return wave_range_of(request_range(a, kind, sp, RowPos{seq, t0, 0}), request_range(a, kind, sp, RowPos{seq, t1, 0}), r);
 }
 
 // Over the 32 rows of a wave (both halves hold them): four exchanges inside 16 lanes, and two lanes read.
@@ -583,7 +599,8 @@ __device__ __forceinline__ void rows_alone(const MaskArgs& a, const RowOut& to, 
         for (int i = 0; i < 2; i++) {
             if (i >= to.job.spans) break;
             const KeySpan& sp = to.job.span[i];
-            const Range r = row_range(a, to.job.kind[i], sp, row_pos(a, to.job, to.it.seq, row0 + x));
+            const RowPos p = row_pos(a, to.job, to.it.seq, row0 + x);
+            const Range r = to.job.kind[i] != kRangeDocs ? request_range(a, to.job.kind[i], sp, p) : range_in(a, doc_of_row(a, p.seq, p.tok, sp.keys, true), p.tok);
             row_alone<F16, MODE>(a, sp, span_base(sp, to.it.seq, to.it.kvh), q, max(r.lo, first[i]), min(r.hi, end[i]), r.pos, sl, lane, m, l, o0, o1);
         }
         if (a.direct) {
@@ -611,19 +628,19 @@ __device__ __forceinline__ void lane_offsets(int lane, FragLane& fl) {
 // Rows [first, end) of the w-th tile of a sequence whose tiles keep to their documents: those of the longest documents
 // first, a document's last first. False: there are fewer tiles. (Documents of 196 to 1373 tokens, 24 heads, 6007 tokens: 114 us
 // with tiles that cross borders and walk the keys of both sides.)
-__device__ __forceinline__ bool tile_of_documents(const MaskArgs& a, int seq, int w, int lane, int& first, int& end) {
+__device__ __forceinline__ bool tile_of_documents(const MaskArgs& a, int seq, int w, int lane, int& first, int& end, int& d) {
     const unsigned* const qb = a.q_starts + (int64_t)seq * (a.documents + 1);
     const unsigned q_tokens = (unsigned)a.q_tokens;
     const int s = (int)min(qb[min(lane, a.documents)], q_tokens), e = (int)min(qb[min(lane + 1, a.documents)], q_tokens);
     const int tiles = lane < a.documents && e > s ? ((e - s) * a.group + kMaskRowsByWave - 1) / kMaskRowsByWave : 0;
     int before = 0; // tiles of documents that come ahead of this lane's
-    for (int d = 0; d < a.documents; d++) {
-        const int t = __builtin_amdgcn_readlane(tiles, d);
-        before += t > tiles || (t == tiles && d < lane) ? t : 0;
+    for (int x = 0; x < a.documents; x++) {
+        const int t = __builtin_amdgcn_readlane(tiles, x);
+        before += t > tiles || (t == tiles && x < lane) ? t : 0;
     }
     const unsigned long long mine = __builtin_amdgcn_ballot_w64(before <= w && w < before + tiles);
     if (mine == 0) return false;
-    const int d = __builtin_ctzll(mine);
+    d = __builtin_ctzll(mine);
     const int t = __builtin_amdgcn_readlane(tiles, d) - 1 - (w - __builtin_amdgcn_readlane(before, d));
     first = __builtin_amdgcn_readlane(s, d) * a.group + t * kMaskRowsByWave;
     end = __builtin_amdgcn_readlane(e, d) * a.group;
@@ -652,8 +669,8 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
     const MaskJob& job = a.job[which];
     const Item it = item_of(a, job, (int)blockIdx.x);
     const RowOut to(a, job, it, kMaskRowsByWave);
-    int tile_row = it.tile * kMaskRowsByWave, row_end = job.rows;
-    if (job.by_document && !tile_of_documents(a, it.seq, job.row_tiles - 1 - it.tile, lane, tile_row, row_end)) return;
+    int tile_row = it.tile * kMaskRowsByWave, row_end = job.rows, doc_no = 0;
+    if (job.by_document && !tile_of_documents(a, it.seq, job.row_tiles - 1 - it.tile, lane, tile_row, row_end, doc_no)) return;
     const int row0 = tile_row + 32 * wave;
     const int row = min(row0 + l32, row_end - 1); // rows past the end work on the last one and are not written
     const RowPos rp = row_pos(a, job, it.seq, row);
@@ -662,9 +679,17 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
     const float c = MODE == kCap ? 1.0f : a.scale_log2;
 
     const char* const qrow = a.q + (int64_t)rp.seq * a.q_ss + (int64_t)rp.tok * a.q_ts + (int64_t)head * a.q_hs;
-    bf16x8 qf[8];
+    // The wave's query rows go through its quarter of the idle V ring, four whole rows a load (a lane that fetches its own row
+    // touches a cache line per lane and load).
 #pragma unroll
-    for (int s = 0; s < 8; s++) qf[s] = *reinterpret_cast<const bf16x8*>(qrow + 32 * s + 16 * h);
+    for (int n = 0; n < 8; n++) {
+        const int from = 4 * (4 * n + (lane >> 4)); // the lane that has the row's address
+        const unsigned long long at = (unsigned long long)(unsigned)__builtin_amdgcn_ds_bpermute(from, (int)(unsigned)(unsigned long long)qrow) |
+                                      (unsigned long long)(unsigned)__builtin_amdgcn_ds_bpermute(from, (int)(unsigned)((unsigned long long)qrow >> 32)) << 32;
+        row_to_lds(reinterpret_cast<const char*>(at) + k_chunk(lane, n), lds0 + kV + (unsigned)wave * (unsigned)kBlock + (unsigned)n * 1024u);
+    }
+    bf16x8 qf[8];
+    bool have_q = false;
     FragLane fl;
     lane_offsets(lane, fl);
 #pragma unroll
@@ -685,9 +710,10 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
 #pragma clang loop unroll(disable)
     for (int i = 0; i < job.spans; i++) {
         const KeySpan& sp = job.span[i];
-        const Range r = row_range(a, job.kind[i], sp, rp);
+        const Doc doc = job.kind[i] != kRangeDocs ? Doc{0, 0, 0, 0, 0} : job.by_document ? doc_at(a, it.seq, doc_no, sp.keys) : a.q_starts ? Doc{0, 0, 0, 0, 0} : doc_of_row(a, it.seq, 0, sp.keys, true);
+        const Range r = lane_range(a, job, job.kind[i], sp, rp, doc);
         live = r.live;
-        const WaveRange wr = wave_range(a, job, job.kind[i], sp, it.seq, min(row0, row_end - 1), min(row0 + 31, row_end - 1), r);
+        const WaveRange wr = wave_range(a, job, job.kind[i], sp, it.seq, min(row0, row_end - 1), min(row0 + 31, row_end - 1), r, doc);
         const int all_lo = __builtin_amdgcn_readfirstlane(wr.all_lo), all_hi = __builtin_amdgcn_readfirstlane(wr.all_hi);
         const RowBias rb{slope, r.pos, __builtin_amdgcn_readfirstlane(wr.pos_lo), __builtin_amdgcn_readfirstlane(wr.pos_hi),
                          a.causal && !a.prefix && job.kind[i] != kRangePrefix};
@@ -758,14 +784,24 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
                 load_rows<true>(sp, base, ln, j + 8 * wave + 4, last, 2 * wave + 1, at - (unsigned)wave * 2048u);
             }
         };
-        // P(-1) = 0 meets the V stage of "block -1", which has to hold finite numbers
-        for (int z = tid; z < kBlock / 16; z += 256) *reinterpret_cast<u32x4*>(smem + kV + (kStages - 1) * kBlock + 16 * z) = u32x4{0u, 0u, 0u, 0u};
         fetch_k(0);
         fetch_k(1);
+        if (!have_q) {
+            wait_loads<4>();
+#pragma unroll
+            for (int t = 0; t < 8; t++) {
+                qf[t] = k_frag(kV + (unsigned)wave * (unsigned)kBlock, fl, t);
+                pin(qf[t]);
+            }
+            have_q = true;
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
         fetch_k(2);
         fetch_v(0);
         fetch_k(3);
         fetch_v(1);
+        // P(-1) = 0 meets the V stage of "block -1", which has to hold finite numbers
+        for (int z = tid; z < kBlock / 16; z += 256) *reinterpret_cast<u32x4*>(smem + kV + (kStages - 1) * kBlock + 16 * z) = u32x4{0u, 0u, 0u, 0u};
         asm volatile("s_waitcnt vmcnt(10) lgkmcnt(0)\n\ts_barrier" : : : "memory");
         f32x16 s_a, s_b;
         bf16x8 p_a[2], p_b[2];
@@ -872,6 +908,7 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
         }
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory"); // the rings are free again
     }
+    if (!have_q) wait_loads<0>(); // (no keys at all: the rows may not arrive in LDS behind the workgroup's end)
     st.l = pair_sum(st.l);
 
     // ---- the rows leave: through LDS, so that they are stored as whole rows
@@ -969,9 +1006,10 @@ __global__ void __launch_bounds__(256, 2) attn_keys_kernel(const MaskArgs a, con
 #pragma clang loop unroll(disable)
     for (int i = 0; i < job.spans; i++) {
         const KeySpan& sp = job.span[i];
-        const Range r = row_range(a, job.kind[i], sp, rp);
+        const Doc doc = job.kind[i] == kRangeDocs && !a.q_starts ? doc_of_row(a, it.seq, 0, sp.keys, true) : Doc{0, 0, 0, 0, 0};
+        const Range r = lane_range(a, job, job.kind[i], sp, rp, doc);
         live = r.live;
-        const WaveRange wr = wave_range(a, job, job.kind[i], sp, it.seq, row0, min(row0 + 31, job.rows - 1), r);
+        const WaveRange wr = wave_range(a, job, job.kind[i], sp, it.seq, row0, min(row0 + 31, job.rows - 1), r, doc);
         const int all_lo = __builtin_amdgcn_readfirstlane(wr.all_lo), all_hi = __builtin_amdgcn_readfirstlane(wr.all_hi);
         const RowBias rb{slope, r.pos, __builtin_amdgcn_readfirstlane(wr.pos_lo), __builtin_amdgcn_readfirstlane(wr.pos_hi),
                          a.causal && !a.prefix && job.kind[i] != kRangePrefix};
