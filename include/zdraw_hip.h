@@ -441,7 +441,7 @@ typedef struct ZdrawHipMaskedAttn {
     uint32_t causal;
     uint32_t documents; /* packed documents of a segment; 0 = the segment is one */
     float scale;        /* 0 = 1 / sqrt(head_dim) */
-    float softcap;      /* 0 = none */
+    float softcap;      /* 0 = none; 2^-10 to 2^10 */
     uint32_t reserved;  /* 0 */
 } ZdrawHipMaskedAttn;
 

@@ -340,18 +340,23 @@ __device__ __forceinline__ bf16x8 round8(const T& p, int at) {
 }
 
 // What becomes of a product q.k before the softmax.
-enum ScoreMode : int { kPlain = 0, kBias = 1, kCap = 2 }; // kCap: and biased, by a slope that may be 0
+enum ScoreMode : int { kPlain = 0, kBias = 1, kCap = 2, kCapBias = 3 };
+constexpr bool has_bias(int mode) { return (mode & 1) != 0; }
+constexpr bool has_cap(int mode) { return (mode & 2) != 0; }
 
-// A capped score, log2: cap tanh(s / cap). tanh x = 1 - 2 / (e^2x + 1) is 1 and -1 at the infinities and NaN at NaN; near 0 it is
-// off by 2^-24 of the cap.
-__device__ __forceinline__ float capped(const MaskArgs& a, float dot) {
-    return __builtin_fmaf(-2.0f * a.cap_out, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(dot * a.cap_in) + 1.0f), a.cap_out);
-}
+// A capped score, log2, is cap tanh(s / cap) = cap - 2 cap r with r = 1 / (e^2x + 1): 1 and -1 caps at the infinities, NaN at NaN;
+// near 0 it is off by 2^-24 of the cap. A block keeps r in the place of the product, the exponential's fma does the rest.
+__device__ __forceinline__ float cap_r(const MaskArgs& a, float dot) { return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(dot * a.cap_in) + 1.0f); }
+// What scales a block's scores there, and what a key that is not seen holds.
+template <int MODE>
+__device__ __forceinline__ float score_scale(const MaskArgs& a) { return has_cap(MODE) ? -2.0f * a.cap_out : a.scale_log2; }
+template <int MODE>
+constexpr float unseen() { return has_cap(MODE) ? INFINITY : -INFINITY; }
 // A score of one key by itself, log2.
 template <int MODE>
 __device__ __forceinline__ float score_of(const MaskArgs& a, float dot, float slope, float dist) {
-    const float y = MODE == kCap ? capped(a, dot) : dot * a.scale_log2;
-    return MODE == kPlain ? y : __builtin_fmaf(-slope, fabsf(dist), y);
+    const float y = has_cap(MODE) ? __builtin_fmaf(-2.0f * a.cap_out, cap_r(a, dot), a.cap_out) : dot * a.scale_log2;
+    return has_bias(MODE) ? __builtin_fmaf(-slope, fabsf(dist), y) : y;
 }
 
 // The bias over a block of keys. From the row's place on one side of the block its distance is linear in the key, and
@@ -361,25 +366,25 @@ struct BiasLine {
     float step, at;
 };
 struct RowBias {
-    float slope;      // log2(e) x the head's; 0 without a bias
+    float slope;      // log2(e) x the head's
     int pos;          // where the row stands
     int pos_lo, pos_hi; // of all rows of the wave
     bool ahead;       // no row sees a key behind itself
 };
 template <int MODE>
-__device__ __forceinline__ BiasLine bias_line(const RowBias& rb, int j0, int h) {
-    BiasLine line{0.f, 0.f};
-    if constexpr (MODE != kPlain) {
+__device__ __forceinline__ BiasLine bias_line(const MaskArgs& a, const RowBias& rb, int j0, int h) {
+    BiasLine line{0.f, has_cap(MODE) ? a.cap_out : 0.f};
+    if constexpr (has_bias(MODE)) {
         line.step = !rb.ahead && j0 >= rb.pos_hi ? -rb.slope : rb.slope;
-        line.at = -line.step * (float)(rb.pos - j0 - 4 * h);
+        line.at = __builtin_fmaf(-line.step, (float)(rb.pos - j0 - 4 * h), line.at);
     }
     return line;
 }
 // A biased row's scores rise towards where it stands (`pos`, the last of the rows'): its blocks are walked from there, down and then up, so that the
 // reference point is found at once and not moved by every block (16384 causal tokens, 24 heads: 2586 us first to last).
 template <int MODE>
-__device__ __forceinline__ int blocks_down(const MaskArgs& a, int pos, int lo, int nb) {
-    if (MODE == kPlain || !a.slopes || pos < lo) return 0;
+__device__ __forceinline__ int blocks_down(int pos, int lo, int nb) {
+    if (!has_bias(MODE) || pos < lo) return 0;
     return min((pos - lo) / KB + 1, nb);
 }
 __device__ __forceinline__ void bend_block(const RowBias& rb, f32x16& s, float c, int j0, int h) {
@@ -389,39 +394,42 @@ __device__ __forceinline__ void bend_block(const RowBias& rb, f32x16& s, float c
 }
 template <int MODE>
 __device__ __forceinline__ float scaled(float s, float c, const BiasLine& line, int i) {
-    if constexpr (MODE == kPlain) return __builtin_fmaf(s, c, line.at);
-    else return __builtin_fmaf(s, c, __builtin_fmaf(line.step, (float)(8 * (i >> 2) + (i & 3)), line.at));
+    if constexpr (has_bias(MODE)) return __builtin_fmaf(s, c, __builtin_fmaf(line.step, (float)(8 * (i >> 2) + (i & 3)), line.at));
+    else return __builtin_fmaf(s, c, line.at);
 }
 
-// The cap, the bend of the bias and the mask of a block's products. Most blocks of most calls need none of it.
+// The cap and the bend of the bias over a block's products. Most blocks of most calls need neither.
 template <int MODE>
 __device__ __forceinline__ void finish_block(const MaskArgs& a, f32x16& s, float c, const RowBias& rb, int j0, int h) {
-    if constexpr (MODE == kCap) {
+    if constexpr (has_cap(MODE)) {
 #pragma unroll
-        for (int i = 0; i < 16; i++) s[i] = capped(a, s[i]);
+        for (int i = 0; i < 16; i++) s[i] = cap_r(a, s[i]);
     }
-    if constexpr (MODE != kPlain) {
+    if constexpr (has_bias(MODE)) {
         if (!rb.ahead && j0 + KB - 1 > rb.pos_lo && j0 < rb.pos_hi) bend_block(rb, s, c, j0, h);
     }
 }
+template <int MODE>
 __device__ __forceinline__ void mask_block(f32x16& s, int j0, int h, const Range& r) {
     const unsigned n = (unsigned)(r.hi - r.lo);
     const unsigned first = (unsigned)(j0 + 4 * h - r.lo);
 #pragma unroll
-    for (int i = 0; i < 16; i++) s[i] = first + (unsigned)(8 * (i >> 2) + (i & 3)) < n ? s[i] : -INFINITY;
+    for (int i = 0; i < 16; i++) s[i] = first + (unsigned)(8 * (i >> 2) + (i & 3)) < n ? s[i] : unseen<MODE>();
 }
+// The highest score of a row in a block, log2.
 template <int MODE>
 __device__ __forceinline__ float block_max(const f32x16& s, float c, const BiasLine& line) {
-    if constexpr (MODE == kPlain) {
-        float top = fmaxf(s[0], s[1]);
-#pragma unroll
-        for (int i = 2; i < 16; i += 2) top = fmaxf(top, fmaxf(s[i], s[i + 1]));
-        return pair_max(top) * c;
-    } else {
+    if constexpr (has_bias(MODE)) {
         float top = scaled<MODE>(s[0], c, line, 0);
 #pragma unroll
         for (int i = 1; i < 16; i++) top = fmaxf(top, scaled<MODE>(s[i], c, line, i));
         return pair_max(top);
+    } else {
+        auto higher = [](float x, float y) __attribute__((always_inline)) { return has_cap(MODE) ? fminf(x, y) : fmaxf(x, y); };
+        float top = higher(s[0], s[1]);
+#pragma unroll
+        for (int i = 2; i < 16; i += 2) top = higher(top, higher(s[i], s[i + 1]));
+        return pair_max(scaled<MODE>(top, c, line, 0));
     }
 }
 
@@ -675,8 +683,8 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
     const int row = min(row0 + l32, row_end - 1); // rows past the end work on the last one and are not written
     const RowPos rp = row_pos(a, job, it.seq, row);
     const int head = it.kvh * a.group + rp.g;
-    const float slope = (MODE != kPlain && a.slopes) ? a.slopes[head] * 1.4426950408889634f : 0.0f;
-    const float c = MODE == kCap ? 1.0f : a.scale_log2;
+    const float slope = has_bias(MODE) ? a.slopes[head] * 1.4426950408889634f : 0.0f;
+    const float c = score_scale<MODE>(a);
 
     const char* const qrow = a.q + (int64_t)rp.seq * a.q_ss + (int64_t)rp.tok * a.q_ts + (int64_t)head * a.q_hs;
     // The wave's query rows go through its quarter of the idle V ring, four whole rows a load (a lane that fetches its own row
@@ -749,7 +757,7 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
         const unsigned ko0 = lq * (unsigned)sp.k_ts + k_chunk(lane, 2 * wave), ko1 = (lq + 4) * (unsigned)sp.k_ts + k_chunk(lane, 2 * wave + 1);
         const unsigned vo0 = lq * (unsigned)sp.v_ts + v_chunk(lane), vo1 = vo0 + 4 * (unsigned)sp.v_ts;
         const int whole_end = base.table ? 0 : lo + (hi - lo) / KB * KB; // up to here blocks lie in memory as they do in LDS
-        const int n_down = blocks_down<MODE>(a, __builtin_amdgcn_readfirstlane(max(max(s_pos[i][0], s_pos[i][1]), max(s_pos[i][2], s_pos[i][3]))), lo, nb);
+        const int n_down = blocks_down<MODE>(__builtin_amdgcn_readfirstlane(max(max(s_pos[i][0], s_pos[i][1]), max(s_pos[i][2], s_pos[i][3]))), lo, nb);
         auto first_key = [&](int b) __attribute__((always_inline)) { return lo + (b < n_down ? n_down - 1 - b : b) * KB; };
         // (unbiased rows take blocks in their order: the address is carried along)
         const char* k_next = base.k + (int64_t)(lo + 8 * wave) * sp.k_ts;
@@ -760,10 +768,10 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
             const unsigned at = lds_w + (unsigned)(b & (kStages - 1)) * (unsigned)kBlock;
             const int j = first_key(b);
             if (j < whole_end) {
-                const char* const p = MODE == kPlain ? k_next : base.k + (int64_t)(j + 8 * wave) * sp.k_ts;
+                const char* const p = !has_bias(MODE) ? k_next : base.k + (int64_t)(j + 8 * wave) * sp.k_ts;
                 rows_to_lds(p, ko0, at);
                 rows_to_lds(p, ko1, at + 1024u);
-                if (MODE == kPlain) k_next += k_step;
+                if (!has_bias(MODE)) k_next += k_step;
             } else {
                 const int ln = lane_again();
                 load_rows<false>(sp, base, ln, j + 8 * wave, last, 2 * wave, at - (unsigned)wave * 2048u);
@@ -774,10 +782,10 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
             const unsigned at = lds_w + kV + (unsigned)(b & (kStages - 1)) * (unsigned)kBlock;
             const int j = first_key(b);
             if (j < whole_end) {
-                const char* const p = MODE == kPlain ? v_next : base.v + (int64_t)(j + 8 * wave) * sp.v_ts;
+                const char* const p = !has_bias(MODE) ? v_next : base.v + (int64_t)(j + 8 * wave) * sp.v_ts;
                 rows_to_lds(p, vo0, at);
                 rows_to_lds(p, vo1, at + 1024u);
-                if (MODE == kPlain) v_next += v_step;
+                if (!has_bias(MODE)) v_next += v_step;
             } else {
                 const int ln = lane_again();
                 load_rows<true>(sp, base, ln, j + 8 * wave, last, 2 * wave, at - (unsigned)wave * 2048u);
@@ -813,11 +821,11 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
         auto finish_scores = [&](f32x16& s, int b) __attribute__((always_inline)) {
             const int j0 = first_key(b);
             finish_block<MODE>(a, s, c, rb, j0, h);
-            if (!(j0 >= all_lo && j0 + KB <= all_hi)) mask_block(s, j0, h, r);
+            if (!(j0 >= all_lo && j0 + KB <= all_hi)) mask_block<MODE>(s, j0, h, r);
         };
         // The reference point at a block's maximum, where that is higher: what was summed goes by the new one.
         auto raise = [&](const f32x16& s, int b) __attribute__((always_inline)) {
-            const float m = fmaxf(st.m, block_max<MODE>(s, c, bias_line<MODE>(rb, first_key(b), h)));
+            const float m = fmaxf(st.m, block_max<MODE>(s, c, bias_line<MODE>(a, rb, first_key(b), h)));
             const float f = st.m == m ? 1.0f : __builtin_amdgcn_exp2f(st.m - m);
             st.m = m;
             st.l *= f;
@@ -850,7 +858,7 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
 #pragma unroll
             for (int x = 0; x < LA; x++) read(x);
             const int j0 = first_key(b);
-            BiasLine line = bias_line<MODE>(rb, j0, h);
+            BiasLine line = bias_line<MODE>(a, rb, j0, h);
             line.at -= st.m == -INFINITY ? 0.0f : st.m;
             float sum = 0.f, e[16];
             __builtin_amdgcn_sched_barrier(0);
@@ -871,7 +879,7 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
             // a score far above the reference point, a number that is none, or the first block that a row sees
             if (__builtin_amdgcn_ballot_w64(!(sum <= kLimit) || (st.m == -INFINITY && r.lo < j0 + KB && r.hi > j0)) != 0) {
                 raise(s, b);
-                line = bias_line<MODE>(rb, j0, h);
+                line = bias_line<MODE>(a, rb, j0, h);
                 line.at -= st.m == -INFINITY ? 0.0f : st.m;
                 sum = 0.f;
 #pragma unroll
@@ -983,8 +991,8 @@ __global__ void __launch_bounds__(256, 2) attn_keys_kernel(const MaskArgs a, con
     const int row = min(row0 + l32, job.rows - 1);
     const RowPos rp = row_pos(a, job, it.seq, row);
     const int head = it.kvh * a.group + rp.g;
-    const float slope = (MODE != kPlain && a.slopes) ? a.slopes[head] * 1.4426950408889634f : 0.0f;
-    const float c = MODE == kCap ? 1.0f : a.scale_log2;
+    const float slope = has_bias(MODE) ? a.slopes[head] * 1.4426950408889634f : 0.0f;
+    const float c = score_scale<MODE>(a);
 
     const char* const qrow = a.q + (int64_t)rp.seq * a.q_ss + (int64_t)rp.tok * a.q_ts + (int64_t)head * a.q_hs;
     bf16x8 qf[8];
@@ -1035,7 +1043,7 @@ __global__ void __launch_bounds__(256, 2) attn_keys_kernel(const MaskArgs a, con
         const unsigned k_off0 = ((unsigned)lane >> 4) * (unsigned)sp.k_ts, v_off0 = ((unsigned)lane >> 4) * (unsigned)sp.v_ts;
         const unsigned k_off[4] = {k_off0 + k_chunk(lane, 0), k_off0 + k_chunk(lane, 1), k_off0 + k_chunk(lane, 2), k_off0 + k_chunk(lane, 3)};
         const unsigned v_off[4] = {v_off0 + v_chunk(lane), 0u, 0u, 0u};
-        const int n_down = blocks_down<MODE>(a, rb.pos_hi, lo, nb);
+        const int n_down = blocks_down<MODE>(rb.pos_hi, lo, nb);
         auto first_key = [&](int b) __attribute__((always_inline)) { return lo + (b < n_down ? n_down - 1 - b : b) * KB; };
         if (wave < nb) {
             load_block<false>(sp, base, lane, k_off, first_key(wave), last, kl);
@@ -1061,9 +1069,9 @@ __global__ void __launch_bounds__(256, 2) attn_keys_kernel(const MaskArgs a, con
 #pragma unroll
             for (int t = 0; t < 8; t++) s = mfma<F16>(kf[t], qf[t], s);
             finish_block<MODE>(a, s, c, rb, j0, h);
-            if (!(j0 >= all_lo && j0 + KB <= all_hi)) mask_block(s, j0, h, r);
+            if (!(j0 >= all_lo && j0 + KB <= all_hi)) mask_block<MODE>(s, j0, h, r);
             bf16x8 p[2];
-            softmax_block<F16, MODE>(s, c, bias_line<MODE>(rb, j0, h), st, p);
+            softmax_block<F16, MODE>(s, c, bias_line<MODE>(a, rb, j0, h), st, p);
             if (more) wait_loads<8>();
             else wait_loads<0>();
             s16x8 vf[2][4];
@@ -1252,7 +1260,9 @@ hipError_t launch_jobs(const MaskArgs& a, hipStream_t stream) {
 
 template <bool F16>
 hipError_t launch_typed(const MaskArgs& a, hipStream_t stream) {
-    const hipError_t e = a.cap_in != 0.0f ? launch_jobs<F16, msk::kCap>(a, stream) : a.slopes ? launch_jobs<F16, msk::kBias>(a, stream) : launch_jobs<F16, msk::kPlain>(a, stream);
+    const bool cap = a.cap_in != 0.0f;
+    const hipError_t e = a.slopes ? (cap ? launch_jobs<F16, msk::kCapBias>(a, stream) : launch_jobs<F16, msk::kBias>(a, stream))
+                                  : (cap ? launch_jobs<F16, msk::kCap>(a, stream) : launch_jobs<F16, msk::kPlain>(a, stream));
     if (e != hipSuccess || a.direct) return e;
     const MaskJob& last = a.job[a.jobs - 1]; // tiled by sequence
     const int rows = last.seqs * a.kv_heads * last.rows;
@@ -1269,16 +1279,20 @@ hipError_t setup_one() {
     if (e == hipSuccess) e = hipFuncSetAttribute(reinterpret_cast<const void*>(&msk::attn_keys_kernel<F16, MODE>), hipFuncAttributeMaxDynamicSharedMemorySize, msk::kLds);
     return e;
 }
+
+template <bool F16>
+hipError_t setup_typed() {
+    hipError_t e = setup_one<F16, msk::kPlain>();
+    if (e == hipSuccess) e = setup_one<F16, msk::kBias>();
+    if (e == hipSuccess) e = setup_one<F16, msk::kCap>();
+    if (e == hipSuccess) e = setup_one<F16, msk::kCapBias>();
+    return e;
+}
 } // namespace
 
 hipError_t masked_setup() {
-    hipError_t e = setup_one<false, msk::kPlain>();
-    if (e == hipSuccess) e = setup_one<false, msk::kBias>();
-    if (e == hipSuccess) e = setup_one<false, msk::kCap>();
-    if (e == hipSuccess) e = setup_one<true, msk::kPlain>();
-    if (e == hipSuccess) e = setup_one<true, msk::kBias>();
-    if (e == hipSuccess) e = setup_one<true, msk::kCap>();
-    return e;
+    const hipError_t e = setup_typed<false>();
+    return e == hipSuccess ? setup_typed<true>() : e;
 }
 
 int masked_launches(const MaskArgs& a) {

@@ -2044,6 +2044,8 @@ int mask_common(uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t d
     if (causal > 1) return invalid("causal");
     if (!(scale >= 0.0f) || !std::isfinite(scale)) return invalid("scale");
     if (!(softcap >= 0.0f) || !std::isfinite(softcap)) return invalid("softcap");
+    // (a capped score is off by 2^-22 of the cap: beyond 2^10 that would show in a 16-bit output)
+    if (softcap != 0.0f && (softcap > 1024.0f || softcap < 0x1p-10f)) return unavailable("softcap outside of 2^-10 to 2^10");
     if (reserved != 0) return invalid("reserved");
     return ZDRAW_HIP_OK;
 }
