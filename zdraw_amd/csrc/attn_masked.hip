@@ -874,7 +874,7 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
                     p[x >> 3] = round8<F16>(e, x - 7);
                     pin(p[x >> 3]);
                 }
-                __builtin_amdgcn_sched_barrier(0);
+                if ((x & 3) == 3) __builtin_amdgcn_sched_barrier(0);
             }
             // a score far above the reference point, a number that is none, or the first block that a row sees
             if (__builtin_amdgcn_ballot_w64(!(sum <= kLimit) || (st.m == -INFINITY && r.lo < j0 + KB && r.hi > j0)) != 0) {

@@ -1937,23 +1937,33 @@ const float* f32_of(void* handle) { return handle ? static_cast<const float*>(st
 
 constexpr uint32_t kMaskMaxTokens = 1u << 24; // positions and row numbers are exact in f32
 
-// How the rows of a call are laid on workgroups (2 per CU). `split_ok`: there is room for parts.
+// How the rows of a call are laid on workgroups, two of which a CU holds. `keys`: that a row sees on average. `split_ok`: there is
+// room for parts.
+//
+// 32 rows a workgroup whose waves take the keys in turn, or 128 whose waves share them: the first is through a key block in a
+// quarter of the steps and reads the keys four times as often. us, first and second form, 32 query and 8 key heads:
+// 512 causal tokens 12.0, 24.3; 1024 26.3, 35.2; 1500 43.5, 36.2; 256 rows at the end of 4096 keys 36.0, 44.4, of 16384
+// keys 121, 88; eight times 256 tokens (2048 tiles) 33.4, 19.3.
+//
+// Keys are split where workgroups are few, in shares of 256 or more: what the join costs, 4 us, is what 512 keys cost.
+// One row of 8 key heads, us, whole and split: 512 keys 8.5, 9.1; 1024 12.3, 9.5; 1500 17.0, 11.2.
 struct MaskLayout {
     int by_keys, row_tiles, splits;
 };
-MaskLayout mask_layout(int64_t rows, int64_t groups, int64_t keys, int cus, bool split_ok) {
+MaskLayout mask_layout(int64_t rows, int64_t groups, int64_t keys, int cus, bool split_ok, int64_t most = 4096) {
     MaskLayout y;
     const int64_t slots = 2 * (int64_t)cus;
     const int64_t tiles32 = (rows + kMaskRowsByKeys - 1) / kMaskRowsByKeys * groups;
-    y.by_keys = rows <= kMaskRowsByKeys || tiles32 <= slots;
+    y.by_keys = rows <= kMaskRowsByKeys || (tiles32 <= 2 * slots && tiles32 * keys <= most * (int64_t)cus);
     const int tr = y.by_keys ? kMaskRowsByKeys : kMaskRowsByWave;
     y.row_tiles = (int)((rows + tr - 1) / tr);
     const int64_t wgs = y.row_tiles * groups;
-    int64_t s = split_ok ? slots / wgs : 1;
-    s = std::min(s, (keys + 255) / 256);
+    const int64_t s = split_ok && keys >= 768 ? std::min(slots / wgs, keys / 256) : 1;
     y.splits = (int)std::max<int64_t>(1, std::min<int64_t>(s, 64));
     return y;
 }
+// Keys that each of nq rows sees on average of nk.
+int64_t mean_keys(int64_t nq, int64_t nk, bool causal) { return !causal ? nk : nq <= nk ? nk - nq / 2 : nk / 2; }
 
 int64_t job_rows(const MaskJob& j) { return (int64_t)j.workgroups * (j.by_keys ? kMaskRowsByKeys : kMaskRowsByWave); }
 
@@ -1977,7 +1987,8 @@ int plan_masked_jobs(const ZdrawHipMaskedAttn* p, int cus, bool split_ok, MaskAr
     MaskJob& j = a->job[0];
     j.spans = 1;
     j.kind[0] = kRangeDocs;
-    MaskLayout y = mask_layout(rows, (int64_t)p->batch * p->kv_heads, p->k_tokens, cus, split_ok);
+    const int64_t docs = std::max(p->documents, 1u);
+    MaskLayout y = mask_layout(rows, (int64_t)p->batch * p->kv_heads, mean_keys(p->q_tokens / docs, p->k_tokens / docs, p->causal != 0), cus, split_ok);
     // Tiles that keep to their documents: where a document fills one on average (shorter ones share tiles), and a lane of a
     // wave holds each.
     if (!y.by_keys && y.splits == 1 && p->documents > 0 && p->documents < 64 && rows / p->documents >= kMaskRowsByWave) {
@@ -2007,7 +2018,8 @@ int plan_shared_jobs(const ZdrawHipSharedAttn* p, int cus, bool split_ok, MaskAr
         j0.spans = both ? 2 : 1;
         j0.kind[0] = both || p->prefix_tokens != 0 ? kRangePrefix : kRangeOwn;
         j0.kind[1] = kRangeOwn;
-        MaskLayout y = mask_layout(rows, groups, (int64_t)p->prefix_tokens + p->capacity, cus, split_ok && !both);
+        const int64_t mine = mean_keys(p->q_tokens, p->capacity, p->causal != 0);
+        MaskLayout y = mask_layout(rows, groups, p->prefix_tokens + mine, cus, split_ok && !both);
         if ((rc = set_job(&j0, y, (int)p->requests, (int)p->kv_heads, rows, 0)) != ZDRAW_HIP_OK) return rc;
         a->direct = j0.splits == 1;
         *part_rows = a->direct ? 0 : (size_t)job_rows(j0);
@@ -2018,13 +2030,16 @@ int plan_shared_jobs(const ZdrawHipSharedAttn* p, int cus, bool split_ok, MaskAr
     j0.spans = j1.spans = 1;
     j0.kind[0] = kRangePrefix;
     j1.kind[0] = kRangeOwn;
-    MaskLayout y0 = mask_layout(pooled, p->kv_heads, p->prefix_tokens, cus, true);
-    MaskLayout y1 = mask_layout(rows, groups, p->capacity, cus, true);
-    // both are on the GPU at once: the workgroup slots are dealt out by the keys that each walks
-    const int64_t slots = 2 * (int64_t)cus, t0 = y0.row_tiles * (int64_t)p->kv_heads, t1 = y1.row_tiles * groups;
-    const double w0 = (double)t0 * p->prefix_tokens, w1 = (double)t1 * p->capacity;
-    y1.splits = (int)std::clamp<int64_t>((int64_t)((double)slots * w1 / (w0 + w1)) / t1, 1, y1.splits);
-    y0.splits = (int)std::clamp<int64_t>((slots - t1 * y1.splits) / t0, 1, y0.splits);
+    // (the second form is a launch of its own: 64 requests of five rows over 4000 keys 63 us in one, 72 in two)
+    MaskLayout y0 = mask_layout(pooled, p->kv_heads, p->prefix_tokens, cus, true, 6144);
+    MaskLayout y1 = mask_layout(rows, groups, mean_keys(p->q_tokens, p->capacity, p->causal != 0), cus, true);
+    if (y0.by_keys && y1.by_keys) {
+        // one launch: the workgroup slots are dealt out by the keys that each job walks, half of them at least to the prefix
+        const int64_t slots = 2 * (int64_t)cus, t0 = y0.row_tiles * (int64_t)p->kv_heads, t1 = y1.row_tiles * groups;
+        const double w0 = (double)t0 * p->prefix_tokens, w1 = (double)t1 * p->capacity;
+        y1.splits = (int)std::clamp<int64_t>((int64_t)((double)slots * w1 / (w0 + w1)) / t1, 1, y1.splits);
+        y0.splits = (int)std::clamp<int64_t>(std::max(slots - t1 * y1.splits, slots / 2) / t0, 1, y0.splits);
+    }
     if ((rc = set_job(&j0, y0, 1, (int)p->kv_heads, pooled, 1)) != ZDRAW_HIP_OK) return rc;
     if ((rc = set_job(&j1, y1, (int)p->requests, (int)p->kv_heads, rows, 0)) != ZDRAW_HIP_OK) return rc;
     j1.part_base = job_rows(j0);
