@@ -139,12 +139,50 @@ def test_keys_of_another_length(ctx, q, k, heads, kv, causal):
         assert (got[:, :q - k] == 0).all()
 
 
-# many rows, so that the waves share key blocks (128 rows a workgroup): more than 512 tiles of 32 rows
-@pytest.mark.parametrize("causal,docs,prefix,cap,slopes", [(True, None, None, 0.0, False), (False, None, None, 0.0, False), (True, [[200, 1, 0, 350, 90]], [[50, 1, 0, 350, 7]], 0.0, False),
-                                                           (True, None, None, 20.0, True), (False, [[33, 64, 500]], None, 0.0, True)])
-def test_many_rows(ctx, causal, docs, prefix, cap, slopes):
-    say(causal, docs, prefix, cap, slopes)
-    Call(ctx, 650, heads=28, kv=28, causal=causal, docs=docs, prefix=prefix, cap=cap, slopes=slopes).check()
+# many rows, so that the waves share key blocks (128 rows a workgroup): more than 1024 tiles of 32 rows
+MANY = dict(heads=56, kv=56)  # of 650 rows: 1176 tiles
+
+
+@pytest.mark.parametrize("dtype", [hip.BF16, hip.F16])
+@pytest.mark.parametrize("causal,docs,prefix,cap,slopes", [(True, None, None, 0.0, False), (False, None, None, 0.0, False), (True, None, [[400]], 0.0, False),
+                                                           (True, None, None, 20.0, True), (False, None, None, 0.0, True), (True, None, [[300]], 0.0, True),
+                                                           (False, None, None, 9.0, False), (False, None, None, 9.0, True)])
+def test_many_rows(ctx, causal, docs, prefix, cap, slopes, dtype):
+    say(causal, docs, prefix, cap, slopes, dtype)
+    Call(ctx, 650, causal=causal, docs=docs, prefix=prefix, cap=cap, slopes=slopes, dtype=dtype, **MANY).check()
+
+
+# tiles that keep to their documents (128 rows or more on average), of any order of lengths, and tiles that cross them
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("docs,prefix", [([[200, 350]], None), ([[129, 0, 500, 1]], None), ([[33, 64, 500]], None), ([[650]], [[70]]), ([[1, 649]], [[1, 400]]), ([[128, 256, 256]], None),
+                                         ([[5] * 130], None), ([[10] * 65], None), ([[9] * 63], [[i % 11 for i in range(63)]]), ([[0, 0, 0, 640]], None)])
+def test_many_rows_of_documents(ctx, docs, prefix, causal):
+    say(len(docs[0]), docs[0][:5], causal)
+    prefix = prefix if causal else None  # (a prefix is causal)
+    Call(ctx, 650, causal=causal, docs=docs, prefix=prefix, **MANY).check()
+    Call(ctx, 650, causal=causal, docs=docs, prefix=prefix, slopes=True, **MANY).check()
+
+
+def test_many_rows_of_documents_with_other_keys(ctx):
+    Call(ctx, 650, 900, causal=False, docs=[[200, 350]], key_docs=[[0, 700]], **MANY).check()
+    Call(ctx, 650, 300, causal=True, docs=[[200, 350]], key_docs=[[290, 10]], **MANY).check()
+    Call(ctx, 330, batch=2, causal=True, docs=[[130, 200], [0, 300]], **MANY).check()
+
+
+# few key blocks of a workgroup whose waves share them: fewer than its ring holds, whole and ragged
+@pytest.mark.parametrize("keys", [1, 31, 32, 33, 64, 65, 97, 128, 129, 160, 161])
+def test_few_key_blocks_of_many_rows(ctx, keys):
+    say(keys)
+    Call(ctx, 40, keys, batch=48, heads=12, kv=12, causal=False).check()
+    Call(ctx, 40, keys, batch=48, heads=24, kv=12, causal=True, slopes=True).check()
+
+
+# many rows over many keys: parts of 128-row tiles
+def test_parts_of_many_rows(ctx):
+    c = Call(ctx, 128, 8200, heads=8, kv=2, batch=2, causal=True)
+    assert hip.lib().zdraw_hip_attention_masked_workspace(ctx.queue, C.byref(c.p)) > 128 * 8 * 2 * 130 * 4
+    c.check()
+    Call(ctx, 200, 17000, heads=6, kv=2, causal=False, cap=30.0).check()
 
 
 # documents of no, one and many rows, more than a tile holds, rows behind the last; with other numbers of keys; padded segments
@@ -209,7 +247,7 @@ def test_rising_scores(ctx, q, heads, sign):
 
 # what a row does not see may hold anything: later keys, other documents', keys behind the last one, memory behind the keys
 @pytest.mark.parametrize("dtype", [hip.BF16, hip.F16])
-@pytest.mark.parametrize("heads", [2, 120])
+@pytest.mark.parametrize("heads", [2, 120, 240])
 @pytest.mark.parametrize("nan", [float("nan"), float("inf"), -65504.0])
 def test_unseen_keys_hold_anything(ctx, nan, heads, dtype):
     say(nan, heads, dtype)
@@ -234,8 +272,8 @@ def test_numbers_that_are_not_finite_reach_the_rows_that_see_them(ctx):
         c.k[0, 40, 0, 3] = inf[2]
         c.q[0, 10, 1, 3] = inf[2]
 
-    for heads in (2, 90):
-        c = Call(ctx, 50, heads=heads, kv=2, x=plant)
+    for q, heads, kv in ((50, 2, 2), (50, 90, 2), (600, 60, 60)):
+        c = Call(ctx, q, heads=heads, kv=kv, x=plant)
         want, _, _ = c.want()
         assert np.isinf(want).any() and np.isnan(want).any()
         c.check()

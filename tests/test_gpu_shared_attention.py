@@ -122,10 +122,21 @@ def test_requests_over_a_prefix(ctx, requests, q, prefix, capacity, page, heads,
 
 
 # rows that fill workgroups by themselves: they walk the prefix, then their own keys
-@pytest.mark.parametrize("page", [0, 16])
-@pytest.mark.parametrize("causal", [True, False])
-def test_many_rows_walk_both(ctx, causal, page):
-    Shared(ctx, 3, 140, 200, 150, lens=[150, 140, 141], page=page, heads=32, kv=32, causal=causal).check()
+@pytest.mark.parametrize("page", [0, 4, 8, 16, 64])
+@pytest.mark.parametrize("causal,cap,slopes", [(True, 0.0, False), (False, 0.0, False), (True, 12.0, True), (False, 0.0, True)])
+def test_many_rows_walk_both(ctx, causal, cap, slopes, page):
+    d = hip.lib().zdraw_hip_dispatch_count()
+    Shared(ctx, 3, 140, 200, 150, lens=[150, 140, 141], page=page, heads=32, kv=32, causal=causal, cap=cap, slopes=slopes).check()
+    assert hip.lib().zdraw_hip_dispatch_count() - d == 1
+    Shared(ctx, 4, 700, 130, 720, lens=[0, 700, 33, 719], q_lens=[5, 700, 0, 699], page=page, heads=16, kv=16, causal=causal, cap=cap, slopes=slopes).check()
+
+
+# the prefix for many requests at once through the form whose waves share key blocks: a launch of its own
+@pytest.mark.parametrize("slopes", [False, True])
+def test_rows_of_many_requests_share_key_blocks(ctx, slopes):
+    d = hip.lib().zdraw_hip_dispatch_count()
+    Shared(ctx, 70, 1, 24000, 20, lens=[(7 * r) % 21 for r in range(70)], q_lens=[r % 3 != 1 for r in range(70)], page=4, heads=32, kv=1, slopes=slopes).check()
+    assert hip.lib().zdraw_hip_dispatch_count() - d == 3  # the prefix, the requests' own keys, the join
 
 
 @pytest.mark.parametrize("causal", [True, False])
