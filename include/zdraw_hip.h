@@ -425,7 +425,7 @@ int zdraw_hip_run_chain_attn_enc(void* batch, const ZdrawHipChainAttnBuffers* bu
  * Q, K, V and the output have one 16-bit type; scores, sums and the running maximum are f32,
  * probabilities are rounded to the type of V. Strides in elements: [0] between segments, [1] between tokens, [2]
  * between heads; multiples of 8, those of the inputs may be 0. Outside of what is described the
- * calls return 1 (head_dim other than 128, f32 operands, 2^24 rows or more) or 2. No queries (q_tokens or
+ * calls return 1 (head_dim other than 128, f32 operands, 2^24 keys or 2^22 query rows of a key head and more) or 2. No queries (q_tokens or
  * batch 0) is no error and enqueues nothing; without keys (k_tokens 0) k and v may be NULL. */
 typedef struct ZdrawHipMaskedAttn {
     uint64_t q_off, k_off, v_off, out_off; /* byte offsets into the buffers, multiples of 16 */
@@ -440,7 +440,7 @@ typedef struct ZdrawHipMaskedAttn {
     uint32_t dtype;     /* ZDRAW_HIP_F16 or ZDRAW_HIP_BF16 */
     uint32_t causal;
     uint32_t documents; /* packed documents of a segment; 0 = the segment is one */
-    float scale;        /* 0 = 1 / sqrt(head_dim) */
+    float scale;        /* 0 = 1 / sqrt(head_dim); 2^-20 to 2^20 */
     float softcap;      /* 0 = none; 2^-10 to 2^10 */
     uint32_t reserved;  /* 0 */
 } ZdrawHipMaskedAttn;

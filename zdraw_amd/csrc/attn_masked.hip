@@ -65,8 +65,8 @@ struct RowPos {
     int seq, tok, g;
 };
 
-// x / d for 0 <= x < 2^24: exact in f32 but for one, which the remainder tells.
-__device__ __forceinline__ int div24(int x, int d) {
+// x / d for 0 <= x < 2^22: the f32 quotient is off by less than one, which the remainder tells.
+__device__ __forceinline__ int div22(int x, int d) {
     int q = (int)((float)x * __builtin_amdgcn_rcpf((float)d));
     const int r = x - q * d;
     q += r >= d ? 1 : 0;
@@ -89,10 +89,10 @@ __device__ __forceinline__ int lane_again() {
 
 __device__ __forceinline__ RowPos row_pos(const MaskArgs& a, const MaskJob& job, int seq, int r) {
     RowPos p;
-    const int t = div24(r, a.group);
+    const int t = div22(r, a.group);
     p.g = r - t * a.group;
     if (job.pooled) {
-        p.seq = div24(t, a.q_tokens);
+        p.seq = div22(t, a.q_tokens);
         p.tok = t - p.seq * a.q_tokens;
     } else {
         p.seq = seq;
@@ -120,13 +120,13 @@ __device__ __forceinline__ Doc doc_at(const MaskArgs& a, int seq, int d, int key
     const const_u32_t qb = (const_u32_t)a.q_starts + (int64_t)seq * (a.documents + 1), kb = (const_u32_t)a.k_starts + (int64_t)seq * (a.documents + 1);
     return doc_of_borders(a, qb[d], qb[d + 1], kb[d], kb[d + 1], a.prefix ? ((const_u32_t)a.prefix)[(int64_t)seq * a.documents + d] : 0u, keys);
 }
-// The document that a row lies in. `ascending`: the lanes' rows ascend by less than 32 inside one sequence; then a lane
-// holds each of up to 63 documents' borders, all loaded in one round trip, and few are looked at.
-__device__ __forceinline__ Doc doc_of_row(const MaskArgs& a, int seq, int tok, int keys, bool ascending) {
+// The document that a row lies in. The rows of a wave's lanes ascend by less than 32 inside one sequence: a lane holds each
+// of up to 63 documents' borders, all loaded in one round trip, and few are looked at.
+__device__ __forceinline__ Doc doc_of_row(const MaskArgs& a, int seq, int tok, int keys) {
     if (!a.q_starts) return doc_of_borders(a, 0u, (unsigned)a.q_tokens, 0u, (unsigned)keys, a.prefix ? ((const_u32_t)a.prefix)[seq] : 0u, keys);
     const unsigned* const qb = a.q_starts + (int64_t)seq * (a.documents + 1);
     int d = 0; // the last border at or below the row
-    if (ascending && a.documents < 64) {
+    if (a.documents < 64) {
         const int lane = lane_again(), mine = min(lane, a.documents);
         const unsigned q = qb[mine], k = a.k_starts[(int64_t)seq * (a.documents + 1) + mine];
         const unsigned pre = a.prefix ? a.prefix[(int64_t)seq * a.documents + min(lane, a.documents - 1)] : 0u;
@@ -202,7 +202,7 @@ __device__ __forceinline__ WaveRange wave_range_of(const Range& first, const Ran
 __device__ __forceinline__ Range lane_range(const MaskArgs& a, const MaskJob& job, int kind, const KeySpan& sp, const RowPos& rp, const Doc& doc) {
     if (kind != kRangeDocs) return request_range(a, kind, sp, rp);
     if (job.by_document || !a.q_starts) return range_in(a, doc, rp.tok);
-    return range_in(a, doc_of_row(a, rp.seq, rp.tok, sp.keys, true), rp.tok);
+    return range_in(a, doc_of_row(a, rp.seq, rp.tok, sp.keys), rp.tok);
 }
 __device__ __forceinline__ WaveRange wave_range(const MaskArgs& a, const MaskJob& job, int kind, const KeySpan& sp, int seq, int first_row, int last_row, const Range& r,
                                                 const Doc& doc) {
@@ -211,7 +211,7 @@ __device__ __forceinline__ WaveRange wave_range(const MaskArgs& a, const MaskJob
         if (a.q_lens || a.slopes) return wave_range_of(r);
         return WaveRange{0, sp.keys, 0, sp.keys, 0, 0};
     }
-    const int t0 = div24(first_row, a.group), t1 = div24(last_row, a.group);
+    const int t0 = div22(first_row, a.group), t1 = div22(last_row, a.group);
     if (kind == kRangeDocs) return wave_range_of(range_in(a, doc, t0), range_in(a, doc, t1), r);
     return wave_range_of(request_range(a, kind, sp, RowPos{seq, t0, 0}), request_range(a, kind, sp, RowPos{seq, t1, 0}), r);
 }
@@ -513,7 +513,9 @@ __device__ void row_alone(const MaskArgs& a, const KeySpan& sp, const SpanBase& 
         l += p;
         o0 = __builtin_fmaf(p, v0, o0);
         o1 = __builtin_fmaf(p, v1, o1);
+        if (l != l) break; // nothing else will come of this row
     }
+    if (l != l) o0 = o1 = l;
 }
 
 template <bool F16>
@@ -540,28 +542,28 @@ __device__ __forceinline__ Item item_of(const MaskArgs& a, const MaskJob& job, i
         // Tile by tile over all heads, the tiles that see the most keys first: the GPU's last workgroups are its shortest. The
         // heads' turn is also the XCDs' where their number is a multiple of 8; tiles that walk the same keys start together
         // and share them in the L2. (Head by head on an XCD, 24 heads of 4096 causal tokens: 126 us, so 109.)
-        const int w = div24(id, sks);
+        const int w = div22(id, sks);
         it.sk = id - w * sks;
-        it.split = div24(w, job.row_tiles);
+        it.split = div22(w, job.row_tiles);
         it.tile = job.row_tiles - 1 - (w - it.split * job.row_tiles);
     } else {
         // The tiles that walk the same share of a head's keys follow each other on one XCD.
         const int groups = sks * job.splits, turns = groups >> 3, idx = id >> 3;
         int group;
         if (idx < turns * job.row_tiles) {
-            const int turn = div24(idx, job.row_tiles);
+            const int turn = div22(idx, job.row_tiles);
             it.tile = idx - turn * job.row_tiles;
             group = turn * 8 + (id & 7);
         } else { // the last few shares, fewer than XCDs, tile by tile
-            const int x = id - 8 * turns * job.row_tiles, g = div24(x, job.row_tiles);
+            const int x = id - 8 * turns * job.row_tiles, g = div22(x, job.row_tiles);
             it.tile = x - g * job.row_tiles;
             group = 8 * turns + g;
         }
         it.tile = job.row_tiles - 1 - it.tile;
-        it.split = div24(group, sks);
+        it.split = div22(group, sks);
         it.sk = group - it.split * sks;
     }
-    it.seq = div24(it.sk, a.kv_heads);
+    it.seq = div22(it.sk, a.kv_heads);
     it.kvh = it.sk - it.seq * a.kv_heads;
     it.tile = __builtin_amdgcn_readfirstlane(it.tile);
     it.sk = __builtin_amdgcn_readfirstlane(it.sk);
@@ -608,7 +610,7 @@ __device__ __forceinline__ void rows_alone(const MaskArgs& a, const RowOut& to, 
             if (i >= to.job.spans) break;
             const KeySpan& sp = to.job.span[i];
             const RowPos p = row_pos(a, to.job, to.it.seq, row0 + x);
-            const Range r = to.job.kind[i] != kRangeDocs ? request_range(a, to.job.kind[i], sp, p) : range_in(a, doc_of_row(a, p.seq, p.tok, sp.keys, true), p.tok);
+            const Range r = to.job.kind[i] != kRangeDocs ? request_range(a, to.job.kind[i], sp, p) : range_in(a, doc_of_row(a, p.seq, p.tok, sp.keys), p.tok);
             row_alone<F16, MODE>(a, sp, span_base(sp, to.it.seq, to.it.kvh), q, max(r.lo, first[i]), min(r.hi, end[i]), r.pos, sl, lane, m, l, o0, o1);
         }
         if (a.direct) {
@@ -718,7 +720,7 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
 #pragma clang loop unroll(disable)
     for (int i = 0; i < job.spans; i++) {
         const KeySpan& sp = job.span[i];
-        const Doc doc = job.kind[i] != kRangeDocs ? Doc{0, 0, 0, 0, 0} : job.by_document ? doc_at(a, it.seq, doc_no, sp.keys) : a.q_starts ? Doc{0, 0, 0, 0, 0} : doc_of_row(a, it.seq, 0, sp.keys, true);
+        const Doc doc = job.kind[i] != kRangeDocs ? Doc{0, 0, 0, 0, 0} : job.by_document ? doc_at(a, it.seq, doc_no, sp.keys) : a.q_starts ? Doc{0, 0, 0, 0, 0} : doc_of_row(a, it.seq, 0, sp.keys);
         const Range r = lane_range(a, job, job.kind[i], sp, rp, doc);
         live = r.live;
         const WaveRange wr = wave_range(a, job, job.kind[i], sp, it.seq, min(row0, row_end - 1), min(row0 + 31, row_end - 1), r, doc);
@@ -1014,7 +1016,7 @@ __global__ void __launch_bounds__(256, 2) attn_keys_kernel(const MaskArgs a, con
 #pragma clang loop unroll(disable)
     for (int i = 0; i < job.spans; i++) {
         const KeySpan& sp = job.span[i];
-        const Doc doc = job.kind[i] == kRangeDocs && !a.q_starts ? doc_of_row(a, it.seq, 0, sp.keys, true) : Doc{0, 0, 0, 0, 0};
+        const Doc doc = job.kind[i] == kRangeDocs && !a.q_starts ? doc_of_row(a, it.seq, 0, sp.keys) : Doc{0, 0, 0, 0, 0};
         const Range r = lane_range(a, job, job.kind[i], sp, rp, doc);
         live = r.live;
         const WaveRange wr = wave_range(a, job, job.kind[i], sp, it.seq, row0, min(row0 + 31, job.rows - 1), r, doc);
@@ -1178,7 +1180,7 @@ __global__ void __launch_bounds__(256) attn_masked_merge_kernel(const MaskArgs a
     const int sk = r / per;
     const int rr = r - sk * per;
     const int seq = sk / a.kv_heads, kvh = sk - seq * a.kv_heads;
-    const int tok = div24(rr, a.group);
+    const int tok = div22(rr, a.group);
     const RowPos p{seq, tok, rr - tok * a.group};
     float m = -INFINITY, l = 0.f;
     f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};

@@ -1913,8 +1913,17 @@ const char* check_rows(void* handle, uint64_t off, const uint64_t* stride, const
         if (n[i] <= 1) continue;
         if (stride[i] % (16 / es) != 0) what = "strides must keep rows 16-byte aligned";
         else if (stride[i] >= (1ull << 58)) what = "stride too large";
-        else if (written && stride[i] < (uint64_t)kHeadDim) what = "rows lie on top of each other";
         last += (unsigned __int128)(n[i] - 1) * stride[i];
+    }
+    if (written && !what) { // from the axis with the smallest stride on, each has to step over what the ones before it span
+        int order[3] = {0, 1, 2};
+        std::sort(order, order + 3, [&](int x, int y) { return stride[x] < stride[y]; });
+        unsigned __int128 span = kHeadDim;
+        for (int i : order) {
+            if (n[i] <= 1) continue;
+            if (stride[i] < span) what = "rows lie on top of each other";
+            span += (unsigned __int128)(n[i] - 1) * stride[i];
+        }
     }
     if (!what && (off > b->len || last * es > b->len - off)) what = "buffer too small for the declared shape";
     if (!what) return nullptr;
@@ -1935,7 +1944,8 @@ bool need_u32(const void* handle, uint64_t count) {
 const unsigned* u32_of(void* handle) { return handle ? static_cast<const unsigned*>(static_cast<Buffer*>(handle)->ptr) : nullptr; }
 const float* f32_of(void* handle) { return handle ? static_cast<const float*>(static_cast<Buffer*>(handle)->ptr) : nullptr; }
 
-constexpr uint32_t kMaskMaxTokens = 1u << 24; // positions and row numbers are exact in f32
+constexpr uint32_t kMaskMaxTokens = 1u << 24; // positions are exact in f32
+constexpr uint64_t kMaskMaxRows = 1u << 22;   // of a key head (and workgroups of a launch): div22 (attn_masked.hip)
 
 // How the rows of a call are laid on workgroups, two of which a CU holds. `keys`: that a row sees on average. `split_ok`: there is
 // room for parts.
@@ -1975,7 +1985,7 @@ int set_job(MaskJob* j, const MaskLayout& y, int seqs, int kv_heads, int64_t row
     j->row_tiles = y.row_tiles;
     j->splits = y.splits;
     const int64_t wgs = (int64_t)seqs * kv_heads * y.row_tiles * y.splits;
-    if (wgs >= (1 << 24)) return unavailable("grid too large");
+    if (wgs >= (int64_t)kMaskMaxRows) return unavailable("grid too large");
     j->workgroups = (int32_t)wgs;
     return ZDRAW_HIP_OK;
 }
@@ -2013,7 +2023,7 @@ int plan_shared_jobs(const ZdrawHipSharedAttn* p, int cus, bool split_ok, MaskAr
     const bool both = p->prefix_tokens != 0 && p->capacity != 0;
     const bool full = rows >= 64 && (rows + 127) / 128 * groups >= cus / 2;
     const int64_t pooled = rows * p->requests;
-    if (!both || !split_ok || full || pooled >= (int64_t)kMaskMaxTokens) {
+    if (!both || !split_ok || full || pooled >= (int64_t)kMaskMaxRows) {
         a->jobs = 1;
         j0.spans = both ? 2 : 1;
         j0.kind[0] = both || p->prefix_tokens != 0 ? kRangePrefix : kRangeOwn;
@@ -2058,6 +2068,7 @@ int mask_common(uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t d
     if (dtype != ZDRAW_HIP_F16 && dtype != ZDRAW_HIP_BF16) return dtype == ZDRAW_HIP_F32 ? unavailable("f32 operands") : invalid("dtype");
     if (causal > 1) return invalid("causal");
     if (!(scale >= 0.0f) || !std::isfinite(scale)) return invalid("scale");
+    if (scale != 0.0f && (scale > 0x1p20f || scale < 0x1p-20f)) return unavailable("scale outside of 2^-20 to 2^20");
     if (!(softcap >= 0.0f) || !std::isfinite(softcap)) return invalid("softcap");
     // (a capped score is off by 2^-22 of the cap: beyond 2^10 that would show in a 16-bit output)
     if (softcap != 0.0f && (softcap > 1024.0f || softcap < 0x1p-10f)) return unavailable("softcap outside of 2^-10 to 2^10");
@@ -2081,7 +2092,7 @@ void mask_scores(MaskArgs* a, uint32_t heads, uint32_t kv_heads, uint32_t dtype,
 int masked_shape(const ZdrawHipMaskedAttn* p) {
     const int rc = mask_common(p->heads, p->kv_heads, p->head_dim, p->dtype, p->causal, p->scale, p->softcap, p->reserved);
     if (rc != ZDRAW_HIP_OK) return rc;
-    if ((uint64_t)p->q_tokens * (p->heads / p->kv_heads) >= kMaskMaxTokens || p->k_tokens >= kMaskMaxTokens) return unavailable("too many tokens");
+    if ((uint64_t)p->q_tokens * (p->heads / p->kv_heads) >= kMaskMaxRows || p->k_tokens >= kMaskMaxTokens) return unavailable("too many tokens");
     if ((uint64_t)p->q_tokens * p->heads * p->batch > 0x7fffffffull || p->batch > 0xffffffu) return unavailable("too many rows");
     if (p->documents > kMaskMaxTokens) return unavailable("too many documents");
     return ZDRAW_HIP_OK;
@@ -2090,7 +2101,7 @@ int masked_shape(const ZdrawHipMaskedAttn* p) {
 int shared_shape(const ZdrawHipSharedAttn* p) {
     const int rc = mask_common(p->heads, p->kv_heads, p->head_dim, p->dtype, p->causal, p->scale, p->softcap, p->reserved);
     if (rc != ZDRAW_HIP_OK) return rc;
-    if ((uint64_t)p->q_tokens * (p->heads / p->kv_heads) >= kMaskMaxTokens || (uint64_t)p->prefix_tokens + p->capacity >= kMaskMaxTokens)
+    if ((uint64_t)p->q_tokens * (p->heads / p->kv_heads) >= kMaskMaxRows || (uint64_t)p->prefix_tokens + p->capacity >= kMaskMaxTokens)
         return unavailable("too many tokens");
     if ((uint64_t)p->q_tokens * p->heads * p->requests > 0x7fffffffull || p->requests > 0xffffffu) return unavailable("too many rows");
     return ZDRAW_HIP_OK;

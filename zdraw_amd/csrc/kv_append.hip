@@ -22,12 +22,12 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {
     const int d0 = lane16 * 8;
     const int slots = a.heads + 2 * a.kv_heads;
     const int chunks = (slots + SLOTS - 1) / SLOTS;
-    const long long group = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
-    const long long token = group / chunks;
-    const int slot0 = (int)(group - token * chunks) * SLOTS;
-    if (token >= (long long)a.requests * a.tokens) return;
-    const int req = (int)(token / a.tokens);
-    const int tok = (int)(token - (long long)req * a.tokens);
+    const unsigned group = blockIdx.x * 16u + (threadIdx.x >> 4); // (rows are fewer than 2^31)
+    const unsigned token = group / (unsigned)chunks;
+    const int slot0 = (int)(group - token * (unsigned)chunks) * SLOTS;
+    const int req = (int)(token / (unsigned)a.tokens);
+    const int tok = (int)(token - (unsigned)req * (unsigned)a.tokens);
+    if (req >= a.requests) return;
 
     Raw8<TIn> raw[SLOTS];
 #pragma unroll
