@@ -558,16 +558,14 @@ class _Wrapped:
     def __init__(self, t):
         from zdraw_amd import hip
 
-        self.t = t
-        self.handle = hip.lib().zdraw_hip_wrap_device_memory(_context().device, t.data_ptr(), t.numel() * t.element_size())
+        self.t, self.lib = t, hip.lib()
+        self.handle = self.lib.zdraw_hip_wrap_device_memory(_context().device, t.data_ptr(), t.numel() * t.element_size())
         if not self.handle:
             raise RuntimeError(hip.last_error())
 
     def __del__(self):
-        from zdraw_amd import hip
-
         if getattr(self, "handle", None):
-            hip.lib().zdraw_hip_release_buffer(self.handle)
+            self.lib.zdraw_hip_release_buffer(self.handle)
             self.handle = None
 
 
