@@ -58,6 +58,13 @@ void zdraw_hip_gemm_launch_rows(uint32_t rows, uint64_t ld, uint32_t k, uint32_t
  * and the bytes of scratch that their shares take. Host arithmetic only. */
 void zdraw_hip_wide_ranges(uint32_t tokens, uint32_t cus, uint32_t* ranges, uint64_t* share_bytes);
 
+/* How the rows of an attention under masks are laid on workgroups on a device with `cus` compute units: `rows` query rows
+ * of a key head (tokens x heads of its group), `groups` = segments x key heads, `keys` that a row sees on average. *tile_rows =
+ * 32 (the waves of a workgroup take the keys in turn) or 128 (they share them); *splits = shares of the keys. Host
+ * arithmetic only. */
+void zdraw_hip_masked_plan(uint64_t rows, uint64_t groups, uint64_t keys, uint32_t cus, uint32_t* tile_rows, uint32_t* row_tiles,
+                           uint32_t* splits);
+
 /* From here on a scratch slot may not grow past `bytes`: what a call does when the device has no
  * more memory. 0 = no limit (default). */
 void zdraw_hip_set_scratch_limit(size_t bytes);

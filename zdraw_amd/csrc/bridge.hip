@@ -2581,6 +2581,16 @@ void zdraw_hip_wide_ranges(uint32_t tokens, uint32_t cus, uint32_t* ranges, uint
     if (share_bytes) *share_bytes = ok ? wide_part_bytes((int)tokens, n) : 0;
 }
 
+void zdraw_hip_masked_plan(uint64_t rows, uint64_t groups, uint64_t keys, uint32_t cus, uint32_t* tile_rows, uint32_t* row_tiles, uint32_t* splits) {
+    if (!tile_rows || !row_tiles || !splits) return;
+    *tile_rows = *row_tiles = *splits = 0;
+    if (rows == 0 || groups == 0 || cus == 0 || rows >= kMaskMaxRows || groups >= (1ull << 31) || keys >= kMaskMaxTokens) return;
+    const MaskLayout y = mask_layout((int64_t)rows, (int64_t)groups, (int64_t)keys, (int)cus, true);
+    *tile_rows = y.by_keys ? kMaskRowsByKeys : kMaskRowsByWave;
+    *row_tiles = (uint32_t)y.row_tiles;
+    *splits = (uint32_t)y.splits;
+}
+
 void zdraw_hip_set_scratch_limit(size_t bytes) { g_scratch_limit = bytes; }
 
 void zdraw_hip_set_gemm_build(int build) { gemm_set_build(build); }
