@@ -101,29 +101,40 @@ __device__ __forceinline__ RowPos row_pos(const MaskArgs& a, const MaskJob& job,
     return p;
 }
 
-// A document: its query rows [qs, qe), keys [ks, ke), and how many of those all of its rows see.
-struct Doc {
-    int qs, qe, ks, ke, pre;
+// What the rows of a document (or of a request) see of a span: row t of [qs, qe) stands on key t + off of nk and sees the
+// first max(pre, min(t + off + 1, nk)) of them, counted from lo; all of them where pre = nk.
+struct Seen {
+    int qs, qe, lo, nk, off, pre;
 };
-// (borders held to the sequence)
-__device__ __forceinline__ Doc doc_of_borders(const MaskArgs& a, unsigned q0, unsigned q1, unsigned k0, unsigned k1, unsigned pre, int keys) {
-    Doc d;
+__device__ __forceinline__ Range range_of(const Seen& d, int tok) {
+    Range r;
+    r.live = d.qs <= tok && tok < d.qe;
+    const int at = tok + d.off;
+    r.lo = d.lo;
+    r.hi = d.lo + (r.live ? max(max(min(at + 1, d.nk), d.pre), 0) : 0);
+    r.pos = d.lo + at;
+    return r;
+}
+
+// A document between borders, which are held to the sequence; the last query stands on the last key.
+__device__ __forceinline__ Seen seen_between(const MaskArgs& a, unsigned q0, unsigned q1, unsigned k0, unsigned k1, unsigned pre, int keys) {
+    Seen d;
     d.qe = (int)min(q1, (unsigned)a.q_tokens);
-    d.qs = min((int)min(q0, (unsigned)a.q_tokens), d.qe);
-    d.ks = (int)min(k0, (unsigned)keys);
-    d.ke = max((int)min(k1, (unsigned)keys), d.ks);
-    d.pre = (int)min(pre, (unsigned)(d.ke - d.ks));
+    d.qs = (int)min(q0, (unsigned)d.qe);
+    d.lo = (int)min(k0, (unsigned)keys);
+    d.nk = max((int)min(k1, (unsigned)keys) - d.lo, 0);
+    d.off = d.nk - d.qe;
+    d.pre = a.causal ? (int)min(pre, (unsigned)d.nk) : d.nk;
     return d;
 }
 // The d-th document of a sequence; d may differ from lane to lane.
-__device__ __forceinline__ Doc doc_at(const MaskArgs& a, int seq, int d, int keys) {
+__device__ __forceinline__ Seen seen_in_document(const MaskArgs& a, int seq, int d, int keys) {
     const const_u32_t qb = (const_u32_t)a.q_starts + (int64_t)seq * (a.documents + 1), kb = (const_u32_t)a.k_starts + (int64_t)seq * (a.documents + 1);
-    return doc_of_borders(a, qb[d], qb[d + 1], kb[d], kb[d + 1], a.prefix ? ((const_u32_t)a.prefix)[(int64_t)seq * a.documents + d] : 0u, keys);
+    return seen_between(a, qb[d], qb[d + 1], kb[d], kb[d + 1], a.prefix ? ((const_u32_t)a.prefix)[(int64_t)seq * a.documents + d] : 0u, keys);
 }
 // The document that a row lies in. The rows of a wave's lanes ascend by less than 32 inside one sequence: a lane holds each
 // of up to 63 documents' borders, all loaded in one round trip, and few are looked at.
-__device__ __forceinline__ Doc doc_of_row(const MaskArgs& a, int seq, int tok, int keys) {
-    if (!a.q_starts) return doc_of_borders(a, 0u, (unsigned)a.q_tokens, 0u, (unsigned)keys, a.prefix ? ((const_u32_t)a.prefix)[seq] : 0u, keys);
+__device__ __forceinline__ Seen seen_by_row(const MaskArgs& a, int seq, int tok, int keys) {
     const unsigned* const qb = a.q_starts + (int64_t)seq * (a.documents + 1);
     int d = 0; // the last border at or below the row
     if (a.documents < 64) {
@@ -137,8 +148,8 @@ __device__ __forceinline__ Doc doc_of_row(const MaskArgs& a, int seq, int tok, i
             if (__builtin_amdgcn_ballot_w64(border <= (unsigned)tok) == 0) break;
             d = border <= (unsigned)tok ? x : d;
         }
-        return doc_of_borders(a, (unsigned)__shfl((int)q, d), (unsigned)__shfl((int)q, d + 1), (unsigned)__shfl((int)k, d), (unsigned)__shfl((int)k, d + 1),
-                              (unsigned)__shfl((int)pre, d), keys);
+        return seen_between(a, (unsigned)__shfl((int)q, d), (unsigned)__shfl((int)q, d + 1), (unsigned)__shfl((int)k, d), (unsigned)__shfl((int)k, d + 1),
+                            (unsigned)__shfl((int)pre, d), keys);
     }
     int top = a.documents;
     while (top - d > 1) {
@@ -146,39 +157,27 @@ __device__ __forceinline__ Doc doc_of_row(const MaskArgs& a, int seq, int tok, i
         if (qb[mid] <= (unsigned)tok) d = mid;
         else top = mid;
     }
-    return doc_at(a, seq, d, keys);
+    return seen_in_document(a, seq, d, keys);
 }
-
-__device__ __forceinline__ Range range_in(const MaskArgs& a, const Doc& d, int tok) {
-    Range r;
-    r.live = d.qs <= tok && tok < d.qe;
-    const int nk = d.ke - d.ks;
-    const int at = tok - d.qs + nk - (d.qe - d.qs); // the last query stands on the last key
-    const int n = a.causal ? max(min(at + 1, nk), d.pre) : nk;
-    r.lo = d.ks;
-    r.hi = d.ks + (r.live ? max(n, 0) : 0);
-    r.pos = d.ks + at;
-    return r;
-}
-
-// The keys of a row that sees the shared prefix, or its request's own.
-__device__ __forceinline__ Range request_range(const MaskArgs& a, int kind, const KeySpan& sp, const RowPos& p) {
-    Range r;
-    r.lo = 0;
+// What a request's rows see of the shared prefix, or of their own keys.
+__device__ __forceinline__ Seen seen_by_request(const MaskArgs& a, int kind, int keys, int seq) {
+    Seen d;
     // (of the prefix, what a request holds itself counts for the bias alone)
-    const int n = a.lens && (kind != kRangePrefix || a.slopes) ? (int)min(((const_u32_t)a.lens)[p.seq], (unsigned)a.own_keys) : 0;
-    const int ql = a.q_lens ? (int)min(((const_u32_t)a.q_lens)[p.seq], (unsigned)a.q_tokens) : a.q_tokens;
-    r.live = p.tok < ql;
-    const int at = p.tok + n - ql;
-    if (kind == kRangePrefix) {
-        r.hi = sp.keys;
-        r.pos = sp.keys + at;
-    } else {
-        r.hi = a.causal ? max(min(at + 1, n), 0) : n;
-        r.pos = at;
-    }
-    if (!r.live) r.hi = 0;
-    return r;
+    const int n = a.lens && (kind != kRangePrefix || a.slopes) ? (int)min(((const_u32_t)a.lens)[seq], (unsigned)a.own_keys) : 0;
+    d.qs = 0;
+    d.qe = a.q_lens ? (int)min(((const_u32_t)a.q_lens)[seq], (unsigned)a.q_tokens) : a.q_tokens;
+    d.lo = 0;
+    d.nk = kind == kRangePrefix ? keys : n;
+    d.off = (kind == kRangePrefix ? keys : 0) + n - d.qe;
+    d.pre = kind == kRangePrefix || !a.causal ? d.nk : 0;
+    return d;
+}
+// One for all rows of a sequence, or of a document that a tile keeps to; otherwise (false) it differs from row to row.
+__device__ __forceinline__ bool one_for_all(const MaskArgs& a, const MaskJob& job, int kind) { return kind == kRangeDocs ? job.by_document || !a.q_starts : !job.pooled; }
+__device__ __forceinline__ Seen seen_by_all(const MaskArgs& a, const MaskJob& job, int kind, int keys, int seq, int document) {
+    if (kind != kRangeDocs) return seen_by_request(a, kind, keys, seq);
+    if (job.by_document) return seen_in_document(a, seq, document, keys);
+    return seen_between(a, 0u, (unsigned)a.q_tokens, 0u, (unsigned)keys, a.prefix ? ((const_u32_t)a.prefix)[seq] : 0u, keys);
 }
 
 // What the rows of a wave see together: from the first to the last key of any row, and what every row sees.
@@ -188,32 +187,23 @@ struct WaveRange {
 };
 __device__ __forceinline__ int wave_min(int x);
 __device__ __forceinline__ int wave_max(int x);
-__device__ __forceinline__ WaveRange wave_range_of(const Range& r) {
-    const bool some = r.hi > r.lo;
-    return WaveRange{wave_min(some ? r.lo : 0x7fffffff), wave_max(some ? r.hi : 0), wave_max(r.lo), wave_min(r.hi), wave_min(r.pos), wave_max(r.pos)};
-}
-// The same where ranges only grow from the first row's to the last one's: inside a document, a request or the prefix. (Rows
-// past their request's, behind the last live one, see nothing.)
-__device__ __forceinline__ WaveRange wave_range_of(const Range& first, const Range& last, const Range& r) {
-    const int hi = last.live ? last.hi : wave_max(r.hi);
-    return WaveRange{first.lo, hi, first.lo, last.live ? first.hi : 0, first.pos, last.pos};
-}
-// Rows [first_row, last_row] of a wave, r its lanes' own (doc: of its rows, where it is one).
-__device__ __forceinline__ Range lane_range(const MaskArgs& a, const MaskJob& job, int kind, const KeySpan& sp, const RowPos& rp, const Doc& doc) {
-    if (kind != kRangeDocs) return request_range(a, kind, sp, rp);
-    if (job.by_document || !a.q_starts) return range_in(a, doc, rp.tok);
-    return range_in(a, doc_of_row(a, rp.seq, rp.tok, sp.keys), rp.tok);
-}
-__device__ __forceinline__ WaveRange wave_range(const MaskArgs& a, const MaskJob& job, int kind, const KeySpan& sp, int seq, int first_row, int last_row, const Range& r,
-                                                const Doc& doc) {
-    if (kind == kRangeDocs && a.q_starts && !job.by_document) return wave_range_of(r);
-    if (job.pooled) {
-        if (a.q_lens || a.slopes) return wave_range_of(r);
+// r: a lane's row's; first_row, last_row: of the wave.
+__device__ __forceinline__ WaveRange ranges(const MaskArgs& a, const MaskJob& job, int kind, const KeySpan& sp, const RowPos& rp, int document, int first_row, int last_row,
+                                            Range& r) {
+    if (one_for_all(a, job, kind)) { // ranges only grow from row to row, and rows past the live ones see nothing
+        const Seen d = seen_by_all(a, job, kind, sp.keys, rp.seq, document);
+        r = range_of(d, rp.tok);
+        const Range first = range_of(d, div22(first_row, a.group)), last = range_of(d, div22(last_row, a.group));
+        const int top = range_of(d, min(div22(last_row, a.group), d.qe - 1)).hi;
+        return WaveRange{d.lo, first.live ? top : d.lo, d.lo, last.live ? first.hi : d.lo, first.pos, last.pos};
+    }
+    if (job.pooled && !a.q_lens && !a.slopes) { // the prefix, all of it for all
+        r = Range{0, sp.keys, 0, true};
         return WaveRange{0, sp.keys, 0, sp.keys, 0, 0};
     }
-    const int t0 = div22(first_row, a.group), t1 = div22(last_row, a.group);
-    if (kind == kRangeDocs) return wave_range_of(range_in(a, doc, t0), range_in(a, doc, t1), r);
-    return wave_range_of(request_range(a, kind, sp, RowPos{seq, t0, 0}), request_range(a, kind, sp, RowPos{seq, t1, 0}), r);
+    r = range_of(job.pooled ? seen_by_request(a, kind, sp.keys, rp.seq) : seen_by_row(a, rp.seq, rp.tok, sp.keys), rp.tok);
+    const bool some = r.hi > r.lo;
+    return WaveRange{wave_min(some ? r.lo : 0x7fffffff), wave_max(some ? r.hi : 0), wave_max(r.lo), wave_min(r.hi), wave_min(r.pos), wave_max(r.pos)};
 }
 
 // Over the 32 rows of a wave (both halves hold them): four exchanges inside 16 lanes, and two lanes read.
@@ -605,13 +595,15 @@ __device__ __forceinline__ void rows_alone(const MaskArgs& a, const RowOut& to, 
         const char* const q = to.q(row0 + x);
         float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
         const float sl = lane_f(slope, x);
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            if (i >= to.job.spans) break;
+#pragma clang loop unroll(disable)
+        for (int i = 0; i < to.job.spans; i++) {
             const KeySpan& sp = to.job.span[i];
+            const int kind = to.job.kind[i];
             const RowPos p = row_pos(a, to.job, to.it.seq, row0 + x);
-            const Range r = to.job.kind[i] != kRangeDocs ? request_range(a, to.job.kind[i], sp, p) : range_in(a, doc_of_row(a, p.seq, p.tok, sp.keys), p.tok);
-            row_alone<F16, MODE>(a, sp, span_base(sp, to.it.seq, to.it.kvh), q, max(r.lo, first[i]), min(r.hi, end[i]), r.pos, sl, lane, m, l, o0, o1);
+            const Range r = range_of(kind != kRangeDocs ? seen_by_request(a, kind, sp.keys, p.seq) : a.q_starts ? seen_by_row(a, p.seq, p.tok, sp.keys) : seen_by_all(a, to.job, kind, sp.keys, p.seq, 0),
+                                     p.tok);
+            row_alone<F16, MODE>(a, sp, span_base(sp, to.it.seq, to.it.kvh), q, max(r.lo, i == 0 ? first[0] : first[1]), min(r.hi, i == 0 ? end[0] : end[1]), r.pos, sl, lane, m, l, o0,
+                                 o1);
         }
         if (a.direct) {
             const float inv = l == 0.f ? 0.f : 1.0f / l;
@@ -720,10 +712,9 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
 #pragma clang loop unroll(disable)
     for (int i = 0; i < job.spans; i++) {
         const KeySpan& sp = job.span[i];
-        const Doc doc = job.kind[i] != kRangeDocs ? Doc{0, 0, 0, 0, 0} : job.by_document ? doc_at(a, it.seq, doc_no, sp.keys) : a.q_starts ? Doc{0, 0, 0, 0, 0} : doc_of_row(a, it.seq, 0, sp.keys);
-        const Range r = lane_range(a, job, job.kind[i], sp, rp, doc);
+        Range r;
+        const WaveRange wr = ranges(a, job, job.kind[i], sp, rp, doc_no, min(row0, row_end - 1), min(row0 + 31, row_end - 1), r);
         live = r.live;
-        const WaveRange wr = wave_range(a, job, job.kind[i], sp, it.seq, min(row0, row_end - 1), min(row0 + 31, row_end - 1), r, doc);
         const int all_lo = __builtin_amdgcn_readfirstlane(wr.all_lo), all_hi = __builtin_amdgcn_readfirstlane(wr.all_hi);
         const RowBias rb{slope, r.pos, __builtin_amdgcn_readfirstlane(wr.pos_lo), __builtin_amdgcn_readfirstlane(wr.pos_hi),
                          a.causal && !a.prefix && job.kind[i] != kRangePrefix};
@@ -739,7 +730,7 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
         hi = __builtin_amdgcn_readfirstlane(hi);
         int nb = hi > lo ? (hi - lo + KB - 1) / KB : 0;
         if (job.splits > 1) {
-            const int per = (nb + job.splits - 1) / job.splits;
+            const int per = div22(nb + job.splits - 1, job.splits);
             lo += it.split * per * KB;
             nb = max(min(per, nb - it.split * per), 0);
         }
@@ -1016,17 +1007,16 @@ __global__ void __launch_bounds__(256, 2) attn_keys_kernel(const MaskArgs a, con
 #pragma clang loop unroll(disable)
     for (int i = 0; i < job.spans; i++) {
         const KeySpan& sp = job.span[i];
-        const Doc doc = job.kind[i] == kRangeDocs && !a.q_starts ? doc_of_row(a, it.seq, 0, sp.keys) : Doc{0, 0, 0, 0, 0};
-        const Range r = lane_range(a, job, job.kind[i], sp, rp, doc);
+        Range r;
+        const WaveRange wr = ranges(a, job, job.kind[i], sp, rp, 0, row0, min(row0 + 31, job.rows - 1), r);
         live = r.live;
-        const WaveRange wr = wave_range(a, job, job.kind[i], sp, it.seq, row0, min(row0 + 31, job.rows - 1), r, doc);
         const int all_lo = __builtin_amdgcn_readfirstlane(wr.all_lo), all_hi = __builtin_amdgcn_readfirstlane(wr.all_hi);
         const RowBias rb{slope, r.pos, __builtin_amdgcn_readfirstlane(wr.pos_lo), __builtin_amdgcn_readfirstlane(wr.pos_hi),
                          a.causal && !a.prefix && job.kind[i] != kRangePrefix};
         int lo = __builtin_amdgcn_readfirstlane(wr.lo), hi = __builtin_amdgcn_readfirstlane(wr.hi);
         int nb = hi > lo ? (hi - lo + KB - 1) / KB : 0;
         if (job.splits > 1) {
-            const int per = (nb + job.splits - 1) / job.splits;
+            const int per = div22(nb + job.splits - 1, job.splits);
             lo += it.split * per * KB;
             nb = max(min(per, nb - it.split * per), 0);
         }
