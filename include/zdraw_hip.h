@@ -562,7 +562,8 @@ void zdraw_hip_metrics_reset(void);
 uint64_t zdraw_hip_dispatch_count(void);
 uint64_t zdraw_hip_command_count(void);
 uint64_t zdraw_hip_attn_fallback_count(void);
-uint64_t zdraw_hip_gpu_ns(void); /* device time summed over completed batches / blocking runs */
+uint64_t zdraw_hip_gpu_ns(void); /* device time summed over completed batches / blocking runs (not the blocking runs of attention
+                                  * under masks, over a shared prefix and of the cache append, which record no events) */
 
 /* Attention-kernel trace (the attention bucket of ZDRAW_KLEIN_TRACE,
  * klein/zflux2_resident.zig:443-467): when on, each attention kernel launch is

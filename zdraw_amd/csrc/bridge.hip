@@ -2400,17 +2400,21 @@ int enqueue_kv_append(Queue* qu, void* q, void* k, void* v, void* q_out, void* c
     return ZDRAW_HIP_OK;
 }
 
-// The blocking form of an entry that takes a batch.
+// The blocking form of an entry that takes a batch. It waits for the queue and records no events: between two of them a
+// call of one short kernel takes 18.7 us, without 11.9.
 template <typename Enqueue>
 int run_blocking(void* queue, Enqueue enqueue_on) {
-    void* b = zdraw_hip_batch_begin(queue);
-    if (!b) {
+    Queue* qu = static_cast<Queue*>(queue);
+    if (!qu) {
         set_err("null queue");
         return ZDRAW_HIP_ERR_HANDLE;
     }
-    const int rc = enqueue_on(static_cast<Batch*>(b)->queue);
-    const int rc2 = zdraw_hip_batch_end(b);
-    return rc != ZDRAW_HIP_OK ? rc : rc2;
+    const int rc = enqueue_on(qu);
+    const hipError_t e = hipStreamSynchronize(qu->stream);  // after a refusal too: nothing of the call is left on the queue
+    if (rc != ZDRAW_HIP_OK) return rc;
+    if (e != hipSuccess) return hip_fail(e, "wait");
+    g_command++;
+    return ZDRAW_HIP_OK;
 }
 
 template <typename Enqueue>
