@@ -34,11 +34,10 @@ def rows(q, k, v, seen, pos, scale=None, cap=0.0, slopes=None, key_pos=None):
         return out, absolute
     scale = 1.0 / np.sqrt(D) if not scale else float(np.float32(scale))
     key_pos = np.arange(keys) if key_pos is None else key_pos
-    finite = all(np.isfinite(x).all() for x in (q, k, v))
     with np.errstate(all="ignore"):
         for h in range(heads):
             kh, vh = k[:, h // (heads // kv)], v[:, h // (heads // kv)]
-            if finite:  # all rows at once
+            if all(np.isfinite(x).all() for x in (q[:, h], kh, vh)):  # all rows at once
                 s = (q[:, h] @ kh.T) * scale
                 if cap:
                     s = cap * np.tanh(s / cap)

@@ -186,6 +186,64 @@ def test_parts_of_many_rows(ctx):
 
 
 # documents of no, one and many rows, more than a tile holds, rows behind the last; with other numbers of keys; padded segments
+# a few tiles more than the GPU has units: the last ones are split along their keys, the others write their rows themselves
+@pytest.mark.parametrize("causal,cap,slopes,dtype", [(False, 0.0, False, hip.BF16), (True, 0.0, False, hip.F16), (False, 9.0, False, hip.F16), (True, 0.0, True, hip.BF16), (True, 20.0, True, hip.BF16)])
+@pytest.mark.parametrize("q,heads,kv", [(600, 52, 52), (299, 108, 54)])
+def test_split_tail(ctx, q, heads, kv, causal, cap, slopes, dtype):
+    say(q, heads, kv, causal, cap, slopes, dtype)
+    L = hip.lib()
+    c = Call(ctx, q, 2750, heads=heads, kv=kv, causal=causal, cap=cap, slopes=slopes, dtype=dtype, pad=(8, 0, 16))
+    d = L.zdraw_hip_dispatch_count()
+    n = L.zdraw_hip_attention_masked_workspace(ctx.queue, C.byref(c.p))
+    assert 0 < n <= 14 * 5 * 128 * 130 * 4  # 4 or 14 tiles of 260 or 270, five shares at most
+    first = c.check()
+    assert L.zdraw_hip_dispatch_count() - d == 2
+    room = ctx.buffer(np.full(n, 0xFF, np.uint8))
+    c.o.workspace = room.handle
+    c.clear()
+    assert np.array_equal(c.check("workspace"), first)
+    small = ctx.buffer(np.zeros(n - 16, np.uint8))
+    c.o.workspace = small.handle
+    assert c.rc() == hip.INVALID and "workspace" in hip.last_error()
+
+
+# ... where rows of a split tile meet numbers that are not finite, in one share or in several
+def test_split_tail_of_rows_that_meet_numbers_that_are_not_finite(ctx):
+    def plant(c):
+        inf = rr.bits(np.array([np.inf, -np.inf, np.nan], np.float32), c.dtype)
+        for h in (47, 51):
+            c.v[0, 20, h, 5] = inf[0]
+            c.v[0, 2100, h, 6] = inf[1]
+            c.k[0, 2190, h, 3] = inf[2]  # seen from row 40 on
+        c.q[0, 10, 51, 3] = inf[2]
+
+    c = Call(ctx, 600, 2750, heads=52, kv=52, x=plant)
+    want, _, _ = c.want()
+    assert np.isinf(want).any() and np.isnan(want).any()
+    c.check()
+
+
+def test_replayed_split_tail(ctx):
+    L = hip.lib()
+    c = Call(ctx, 600, 2100, heads=52, kv=52, causal=False)
+    other = Call(ctx, 1, 60000, heads=8, kv=2, seed=5)
+    queue = L.zdraw_hip_create_queue(ctx.device)
+    first = c.check()
+    keep = ctx.buffer(nbytes=L.zdraw_hip_attention_masked_workspace(queue, C.byref(c.p)))
+    for room in (None, keep.handle):
+        c.o.workspace = room
+        g = rr.Captured(queue, c.enqueue)
+        assert g.nodes() == (2 if room else 1)
+        for _ in range(3):
+            c.clear()
+            g.replay()
+            bits = c.check("replayed", run=False) if room is None else c.read()
+            assert room is None or np.array_equal(bits, first)
+            assert other.rc(queue) == 0
+        g.close()
+    L.zdraw_hip_release_queue(queue)
+
+
 @pytest.mark.parametrize("docs,key_docs,batch,q,k", [
     ([[5, 0, 1, 40, 100]], None, 1, 150, 150), ([[1] * 70], None, 1, 70, 70), ([[0, 0]], None, 1, 9, 9), ([[10, 0, 20]], [[3, 5, 0]], 1, 64, 8),
     ([[7, 30]], [[300, 20]], 1, 37, 330), ([[1], [64], [17]], None, 3, 64, 64), ([[100, 28], [0, 77]], [[4, 200], [50, 60]], 2, 128, 260)])

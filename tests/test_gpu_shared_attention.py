@@ -131,6 +131,27 @@ def test_many_rows_walk_both(ctx, causal, cap, slopes, page):
     Shared(ctx, 4, 700, 130, 720, lens=[0, 700, 33, 719], q_lens=[5, 700, 0, 699], page=page, heads=16, kv=16, causal=causal, cap=cap, slopes=slopes).check()
 
 
+# a few workgroups over the GPU's units, or half of its units: the last ones' prefix and own keys are split (and 66 rows of 128
+# workgroups are few enough for the form whose waves take the key blocks in turn)
+@pytest.mark.parametrize("causal,cap,slopes", [(False, 0.0, False), (True, 0.0, False), (True, 12.0, True)])
+@pytest.mark.parametrize("requests,q,kv,page,lens,q_lens", [
+    (2, 66, 64, 0, [200, 131], None), (2, 127, 64, 0, [200, 131], None), (3, 66, 86, 16, [0, 200, 77], [66, 40, 66]),
+    (4, 66, 65, 64, [200, 64, 65, 4000000000], [0, 66, 1, 66])])
+def test_split_tail(ctx, requests, q, kv, page, lens, q_lens, causal, cap, slopes):
+    say(requests, q, kv, page, lens, causal, cap, slopes)
+    c = Shared(ctx, requests, q, 2100, 200, lens=lens, q_lens=q_lens, page=page, heads=kv, kv=kv, causal=causal, cap=cap, slopes=slopes)
+    split = (requests, q) != (2, 66)
+    n = hip.lib().zdraw_hip_attention_shared_workspace(ctx.queue, C.byref(c.p))
+    assert (n > 0) == split
+    d = hip.lib().zdraw_hip_dispatch_count()
+    first = c.check()
+    assert hip.lib().zdraw_hip_dispatch_count() - d == 1 + split
+    room = ctx.buffer(np.full(max(n, 16), 0xFF, np.uint8))
+    c.o.workspace = room.handle
+    c.clear()
+    assert np.array_equal(c.check("workspace"), first)
+
+
 # the prefix for many requests at once through the form whose waves share key blocks: a launch of its own
 @pytest.mark.parametrize("slopes", [False, True])
 def test_rows_of_many_requests_share_key_blocks(ctx, slopes):

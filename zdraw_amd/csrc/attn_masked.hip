@@ -523,12 +523,25 @@ __device__ __forceinline__ unsigned round2(float x, float y) {
 
 // The workgroup's place: sequence, key head, tile of rows, share of the keys.
 struct Item {
-    int sk, seq, kvh, tile, split;
+    int sk, seq, kvh, tile, split, splits;
+    int at; // among the workgroups' parts
+    bool whole; // writes the rows themselves
 };
 __device__ __forceinline__ Item item_of(const MaskArgs& a, const MaskJob& job, int id) {
     const int sks = job.seqs * a.kv_heads;
     Item it;
+    it.splits = job.splits;
+    it.at = 0;
+    it.whole = a.direct;
     if (!job.by_keys) {
+        int share = 0;
+        if (a.direct && id >= job.whole) { // the tail, share by share
+            share = div22(id - job.whole, job.tail);
+            id -= share * job.tail;
+            it.whole = false;
+            it.splits = job.tail_splits;
+            it.at = (id - job.whole) * job.tail_splits + share;
+        }
         // Tile by tile over all heads, the tiles that see the most keys first: the GPU's last workgroups are its shortest. The
         // heads' turn is also the XCDs' where their number is a multiple of 8; tiles that walk the same keys start together
         // and share them in the L2. (Head by head on an XCD, 24 heads of 4096 causal tokens: 126 us, so 109.)
@@ -536,6 +549,7 @@ __device__ __forceinline__ Item item_of(const MaskArgs& a, const MaskJob& job, i
         it.sk = id - w * sks;
         it.split = div22(w, job.row_tiles);
         it.tile = job.row_tiles - 1 - (w - it.split * job.row_tiles);
+        if (a.direct) it.split = share;
     } else {
         // The tiles that walk the same share of a head's keys follow each other on one XCD.
         const int groups = sks * job.splits, turns = groups >> 3, idx = id >> 3;
@@ -553,11 +567,14 @@ __device__ __forceinline__ Item item_of(const MaskArgs& a, const MaskJob& job, i
         it.split = div22(group, sks);
         it.sk = group - it.split * sks;
     }
+    if (!a.direct) it.at = (it.sk * job.row_tiles + it.tile) * job.splits + it.split;
     it.seq = div22(it.sk, a.kv_heads);
     it.kvh = it.sk - it.seq * a.kv_heads;
     it.tile = __builtin_amdgcn_readfirstlane(it.tile);
     it.sk = __builtin_amdgcn_readfirstlane(it.sk);
     it.split = __builtin_amdgcn_readfirstlane(it.split);
+    it.splits = __builtin_amdgcn_readfirstlane(it.splits);
+    it.at = __builtin_amdgcn_readfirstlane(it.at);
     it.seq = __builtin_amdgcn_readfirstlane(it.seq);
     it.kvh = __builtin_amdgcn_readfirstlane(it.kvh);
     return it;
@@ -570,7 +587,7 @@ struct RowOut {
     Item it;
     int64_t part; // first row of the workgroup's parts
     __device__ RowOut(const MaskArgs& args, const MaskJob& j, const Item& i, int tile_rows)
-        : a(args), job(j), it(i), part(j.part_base + ((int64_t)(i.sk * j.row_tiles + i.tile) * j.splits + i.split) * tile_rows) {}
+        : a(args), job(j), it(i), part(j.part_base + (int64_t)i.at * tile_rows) {}
     __device__ __forceinline__ char* out(int row) const {
         const RowPos p = row_pos(a, job, it.seq, row);
         return a.o + (int64_t)p.seq * a.o_ss + (int64_t)p.tok * a.o_ts + (int64_t)(it.kvh * a.group + p.g) * a.o_hs;
@@ -605,7 +622,7 @@ __device__ __forceinline__ void rows_alone(const MaskArgs& a, const RowOut& to, 
             row_alone<F16, MODE>(a, sp, span_base(sp, to.it.seq, to.it.kvh), q, max(r.lo, i == 0 ? first[0] : first[1]), min(r.hi, i == 0 ? end[0] : end[1]), r.pos, sl, lane, m, l, o0,
                                  o1);
         }
-        if (a.direct) {
+        if (to.it.whole) {
             const float inv = l == 0.f ? 0.f : 1.0f / l;
             *reinterpret_cast<unsigned*>(to.out(row0 + x) + 4 * lane) = round2<F16>(o0 * inv, o1 * inv);
         } else {
@@ -729,8 +746,8 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
         lo = __builtin_amdgcn_readfirstlane(lo);
         hi = __builtin_amdgcn_readfirstlane(hi);
         int nb = hi > lo ? (hi - lo + KB - 1) / KB : 0;
-        if (job.splits > 1) {
-            const int per = div22(nb + job.splits - 1, job.splits);
+        if (it.splits > 1) {
+            const int per = div22(nb + it.splits - 1, it.splits);
             lo += it.split * per * KB;
             nb = max(min(per, nb - it.split * per), 0);
         }
@@ -921,7 +938,7 @@ __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, con
         for (int i = 0; i < 16; i++) z = __builtin_fmaf(st.o[b][i], 0.0f, z);
     z = pair_sum(__builtin_fmaf(st.l, 0.0f, z));
     const unsigned bad = (unsigned)__builtin_amdgcn_ballot_w64(here && !(z == 0.0f));
-    if (a.direct) {
+    if (it.whole) {
         const float inv = st.l > 0.f ? 1.0f / st.l : 0.f;
         unsigned char* const mine = smem + wave * (32 * kRow); // (the rings are idle; 16-byte chunks swizzled by row)
 #pragma unroll
@@ -1165,10 +1182,19 @@ __global__ void __launch_bounds__(256) attn_masked_merge_kernel(const MaskArgs a
     const int hw = (int)threadIdx.x >> 5, c = (int)threadIdx.x & 31;
     const int way = hw % WAYS;
     const int r = min((int)blockIdx.x * ROWS + hw / WAYS, rows - 1); // (sequence, key head, row of the sequence)
-    const bool mine = (int)blockIdx.x * ROWS + hw / WAYS < rows;
     const int per = a.q_tokens * a.group;
-    const int sk = r / per;
-    const int rr = r - sk * per;
+    int sk, rr;
+    bool mine = (int)blockIdx.x * ROWS + hw / WAYS < rows;
+    if (a.direct) { // the tail's tiles (a workgroup has rows of one)
+        const Item it = item_of(a, a.job[0], a.job[0].whole + r / kMaskRowsByWave);
+        sk = it.sk;
+        rr = it.tile * kMaskRowsByWave + r % kMaskRowsByWave;
+        mine = mine && rr < per;
+        rr = min(rr, per - 1);
+    } else {
+        sk = r / per;
+        rr = r - sk * per;
+    }
     const int seq = sk / a.kv_heads, kvh = sk - seq * a.kv_heads;
     const int tok = div22(rr, a.group);
     const RowPos p{seq, tok, rr - tok * a.group};
@@ -1189,15 +1215,16 @@ __global__ void __launch_bounds__(256) attn_masked_merge_kernel(const MaskArgs a
         const int row = job.pooled ? seq * per + rr : rr;
         const int at_sk = job.pooled ? kvh : sk;
         const int tile = row / tr;
-        const int64_t at = job.part_base + (int64_t)(at_sk * job.row_tiles + tile) * job.splits * tr + (row - tile * tr);
-        for (int s = way; s < job.splits; s += 4 * WAYS) {
+        const int splits = a.direct ? job.tail_splits : job.splits;
+        const int64_t at = job.part_base + (int64_t)(a.direct ? r / kMaskRowsByWave : at_sk * job.row_tiles + tile) * splits * tr + (row - tile * tr);
+        for (int s = way; s < splits; s += 4 * WAYS) {
             float ml[4][2];
             f32x4 x[4];
 #pragma unroll
             for (int u = 0; u < 4; u++) {
-                const int64_t i = at + (int64_t)min(s + u * WAYS, job.splits - 1) * tr;
+                const int64_t i = at + (int64_t)min(s + u * WAYS, splits - 1) * tr;
                 ml[u][0] = a.part_ml[2 * i];
-                ml[u][1] = s + u * WAYS < job.splits ? a.part_ml[2 * i + 1] : 0.f;
+                ml[u][1] = s + u * WAYS < splits ? a.part_ml[2 * i + 1] : 0.f;
                 x[u] = *reinterpret_cast<const f32x4*>(a.part_o + i * D + 4 * c);
             }
 #pragma unroll
@@ -1255,11 +1282,11 @@ hipError_t launch_typed(const MaskArgs& a, hipStream_t stream) {
     const bool cap = a.cap_in != 0.0f;
     const hipError_t e = a.slopes ? (cap ? launch_jobs<F16, msk::kCapBias>(a, stream) : launch_jobs<F16, msk::kBias>(a, stream))
                                   : (cap ? launch_jobs<F16, msk::kCap>(a, stream) : launch_jobs<F16, msk::kPlain>(a, stream));
-    if (e != hipSuccess || a.direct) return e;
     const MaskJob& last = a.job[a.jobs - 1]; // tiled by sequence
-    const int rows = last.seqs * a.kv_heads * last.rows;
+    if (e != hipSuccess || (a.direct && last.tail == 0)) return e;
+    const int rows = a.direct ? last.tail * kMaskRowsByWave : last.seqs * a.kv_heads * last.rows;
     int parts = 0;
-    for (int i = 0; i < a.jobs; i++) parts += a.job[i].splits;
+    for (int i = 0; i < a.jobs; i++) parts += a.direct ? last.tail_splits : a.job[i].splits;
     if (parts > 4) msk::attn_masked_merge_kernel<F16, 8><<<dim3((unsigned)rows), dim3(256), 0, stream>>>(a, rows);
     else msk::attn_masked_merge_kernel<F16, 1><<<dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, stream>>>(a, rows);
     return hipGetLastError();
@@ -1288,7 +1315,7 @@ hipError_t masked_setup() {
 }
 
 int masked_launches(const MaskArgs& a) {
-    return (a.jobs == 2 && !(a.job[0].by_keys && a.job[1].by_keys) ? 2 : 1) + (a.direct ? 0 : 1);
+    return (a.jobs == 2 && !(a.job[0].by_keys && a.job[1].by_keys) ? 2 : 1) + (a.direct && a.job[0].tail == 0 ? 0 : 1);
 }
 
 hipError_t launch_masked(const MaskArgs& a, hipStream_t stream) { return a.f16 ? launch_typed<true>(a, stream) : launch_typed<false>(a, stream); }

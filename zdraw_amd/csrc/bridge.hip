@@ -1977,6 +1977,8 @@ int64_t mean_keys(int64_t nq, int64_t nk, bool causal) { return !causal ? nk : n
 
 int64_t job_rows(const MaskJob& j) { return (int64_t)j.workgroups * (j.by_keys ? kMaskRowsByKeys : kMaskRowsByWave); }
 
+constexpr int64_t kTailKeys = 1024; // that a split keeps a tile's last workgroup from
+
 int set_job(MaskJob* j, const MaskLayout& y, int seqs, int kv_heads, int64_t rows, int pooled) {
     j->by_keys = y.by_keys;
     j->seqs = seqs;
@@ -1986,9 +1988,28 @@ int set_job(MaskJob* j, const MaskLayout& y, int seqs, int kv_heads, int64_t row
     j->splits = y.splits;
     const int64_t wgs = (int64_t)seqs * kv_heads * y.row_tiles * y.splits;
     if (wgs >= (int64_t)kMaskMaxRows) return unavailable("grid too large");
-    j->workgroups = (int32_t)wgs;
+    j->workgroups = j->whole = (int32_t)wgs;
     return ZDRAW_HIP_OK;
 }
+
+// Tiles of 128 rows that walk `least` keys or more each: where their number is a little over a multiple of the compute
+// units', the last few keep few of them at work. These are walked by as many workgroups as spread each over idle units, 512
+// keys and up a share; so many keys are worth the shares' own start and the merge. Without and with, 24 heads: 1400 rows (264
+// tiles, 8 of them split) 97.9 and 87.5 us for 4096 keys, 43.4 and 41.2 for 1536; 4608 rows (864, 96) 234 and 225 us for
+// 4096 keys, 126 and 125 for 2048. (Twice the shares, for two workgroups a unit: 239 us.)
+size_t set_tail(MaskJob* j, int64_t least, int cus, bool split_ok) {
+    const int tail = j->workgroups % cus;
+    if (!split_ok || j->by_keys || j->by_document || tail == 0) return 0;
+    const int s = (int)std::min<int64_t>(cus / tail, least / 512);
+    if (s < 2 || least * (s - 1) < kTailKeys * s) return 0;
+    j->tail = tail;
+    j->tail_splits = s;
+    j->whole = j->workgroups - tail;
+    j->workgroups = j->whole + tail * s;
+    return (size_t)tail * s * kMaskRowsByWave;
+}
+// Keys that every one of nq rows sees.
+constexpr int64_t fewest_keys(int64_t nq, int64_t nk, bool causal) { return !causal ? nk : std::max<int64_t>(nk - nq, 0); }
 
 // The jobs of a call from its shape alone, and the bytes of room their parts take.
 int plan_masked_jobs(const ZdrawHipMaskedAttn* p, int cus, bool split_ok, MaskArgs* a, size_t* part_rows) {
@@ -2008,7 +2029,8 @@ int plan_masked_jobs(const ZdrawHipMaskedAttn* p, int cus, bool split_ok, MaskAr
     const int rc = set_job(&j, y, (int)p->batch, (int)p->kv_heads, rows, 0);
     if (rc != ZDRAW_HIP_OK) return rc;
     a->direct = j.splits == 1;
-    *part_rows = a->direct ? 0 : (size_t)job_rows(j);
+    *part_rows = !a->direct ? (size_t)job_rows(j)
+               : p->documents != 0 ? 0 : set_tail(&j, fewest_keys(p->q_tokens, p->k_tokens, p->causal != 0), cus, split_ok);
     return ZDRAW_HIP_OK;
 }
 
@@ -2032,7 +2054,7 @@ int plan_shared_jobs(const ZdrawHipSharedAttn* p, int cus, bool split_ok, MaskAr
         MaskLayout y = mask_layout(rows, groups, p->prefix_tokens + mine, cus, split_ok && !both);
         if ((rc = set_job(&j0, y, (int)p->requests, (int)p->kv_heads, rows, 0)) != ZDRAW_HIP_OK) return rc;
         a->direct = j0.splits == 1;
-        *part_rows = a->direct ? 0 : (size_t)job_rows(j0);
+        *part_rows = !a->direct ? (size_t)job_rows(j0) : set_tail(&j0, p->prefix_tokens + fewest_keys(p->q_tokens, p->capacity, p->causal != 0), cus, split_ok);
         return ZDRAW_HIP_OK;
     }
     a->jobs = 2;
@@ -2121,7 +2143,7 @@ int check_pages(uint32_t page_tokens, uint32_t pages, uint32_t capacity, uint32_
 
 // Room for the parts, and the launch.
 int enqueue_masked(Queue* qu, MaskArgs* a, size_t part_rows, void* workspace) {
-    if (!a->direct) {
+    if (part_rows != 0) {
         const size_t ml = part_rows * 2 * sizeof(float), o = part_rows * kHeadDim * sizeof(float);
         if (workspace) {
             const Buffer* w = static_cast<Buffer*>(workspace);

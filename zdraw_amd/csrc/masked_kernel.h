@@ -36,7 +36,9 @@ struct MaskJob {
     int32_t rows;      // per sequence
     int32_t row_tiles, splits;
     int32_t by_document; // 1: tiles keep to the documents, row_tiles is the most that there can be
-    int32_t workgroups; // seqs * kv_heads * row_tiles * splits
+    int32_t workgroups; // seqs * kv_heads * row_tiles * splits, or whole + tail * tail_splits
+    int32_t whole;      // of a direct job of 128-row tiles: so many workgroups write their rows themselves, and behind them
+    int32_t tail, tail_splits; // so many tiles (or none) are walked by tail_splits workgroups each, which leave parts
     int64_t part_base; // first row of this job's parts in part_o / part_ml
 };
 
@@ -60,7 +62,7 @@ struct MaskArgs {
     MaskJob job[2];
     float* part_o;  // [row][128] unnormalised
     float* part_ml; // [row][2]: reference point (log2), denominator
-    int32_t direct; // 1: one job without splits, which writes the output itself
+    int32_t direct; // 1: one job without splits, which writes the output itself, all but its tail's
 };
 
 constexpr int kMaskRowsByWave = 128; // rows of a workgroup whose waves share key blocks
