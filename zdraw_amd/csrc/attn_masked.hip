@@ -674,7 +674,8 @@ __device__ __forceinline__ bool tile_of_documents(const MaskArgs& a, int seq, in
 // the stages that the step before has read for the last time, so one barrier a step orders all of it.
 // A reference point that moves in step b rescales O at its end: what P(b - 1) adds in it still goes by the old one.
 // 24 heads of 8192 rows over all 8192 keys: 743 us, 1110 TFLOP/s, a step of 1440 cycles for 1024 of matrix work at the
-// 1.69 GHz that the power limit leaves; capped 910 us; 16384 causal biased rows 1600 us, 1010 TFLOP/s.
+// 1.69 GHz that the power limit leaves (723 us with 256 rows and eight waves a workgroup, which lose 3 to 6 % on 4608 rows
+// and on causal ones: nobody works in a lone workgroup's start and end); capped 910 us; 16384 causal biased rows 1600 us, 1010 TFLOP/s.
 template <bool F16, int MODE>
 __global__ void __launch_bounds__(256, 2) attn_rows_kernel(const MaskArgs a, const int which) {
     touch_args<sizeof(MaskArgs) + sizeof(int)>();
