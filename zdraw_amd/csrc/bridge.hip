@@ -1996,7 +1996,8 @@ int set_job(MaskJob* j, const MaskLayout& y, int seqs, int kv_heads, int64_t row
 // units', the last few keep few of them at work. These are walked by as many workgroups as spread each over idle units, 512
 // keys and up a share; so many keys are worth the shares' own start and the merge. Without and with, 24 heads: 1400 rows (264
 // tiles, 8 of them split) 97.9 and 87.5 us for 4096 keys, 43.4 and 41.2 for 1536; 4608 rows (864, 96) 234 and 225 us for
-// 4096 keys, 126 and 125 for 2048. (Twice the shares, for two workgroups a unit: 239 us.)
+// 4096 keys, 126 and 125 for 2048. (Twice the shares, for two workgroups a unit: 239 us; the shares ahead of the whole tiles:
+// 129 us for 2048 keys.)
 size_t set_tail(MaskJob* j, int64_t least, int cus, bool split_ok) {
     const int tail = j->workgroups % cus;
     if (!split_ok || j->by_keys || j->by_document || tail == 0) return 0;
